@@ -372,6 +372,61 @@ int otpu_mx_matmul(const double* h, int64_t ldh, const uint8_t* da, int64_t ldda
                    int64_t ldw, const uint8_t* dw, int64_t lddw, int dw_rows, int W, int M, int N, int K,
                    double* y, int64_t ldy, otpu_stream_t stream);
 
+/* ---- between the linears ------------------------------------------------------------------------
+ * What stands between a decoder's quantized linears, for a batch of sequences that share a prompt.  The
+ * reference runs norms and attention as kernels of its own language (opentpu/kernels/); these have no
+ * counterpart of the same form there. */
+
+/* Types of rows and caches. */
+enum { OTPU_F32 = 0, OTPU_BF16 = 1, OTPU_F16 = 2 };
+
+/* The root-mean-square norm in front of a linear, with the residual's addition and the quantizer:
+ *   h = x + res (fp32, res may be NULL), r = 1 / sqrt(mean(h^2) + eps) of the unrounded h, and
+ *   QACT of (h * r) * gamma in groups of 32 (OTPU_Q_ROW: one offset), as otpu_qact with rscale r and
+ *   cscale gamma quantizes the fp32 h, bit for bit.
+ *   x [M, ldx], res [M, ldr], h [M, ldh] of type dtype (OTPU_F32, OTPU_BF16, OTPU_F16); h (may be NULL)
+ *   gets the sum rounded to dtype and may be x or res; gamma [K] fp32; r [M] (may be NULL); q, S, d as
+ *   otpu_qact.  K a multiple of 32, at most OTPU_NORM_COLS.  Rows 16-byte aligned; q's rows 4-byte (16-bit
+ *   types: 8-byte) aligned.  A row whose sum of squares passes fp32's range gives r = 0. */
+#define OTPU_NORM_COLS 32768
+int otpu_norm_qact(const void* x, int64_t ldx, const void* res, int64_t ldr, int dtype, int M, int K,
+                   const float* gamma, float eps, int flags, void* h, int64_t ldh, float* r, int8_t* q,
+                   int64_t ldq, float* S, uint8_t* d, int64_t ldd, otpu_stream_t stream);
+
+/* Attention for a batch that shares a long prefix, which is read and multiplied once for all sequences.
+ *   q [B, Lq, Hq, D] (strides qb, qt, qh in elements, columns adjacent), the prefix's pk, pv [P, Hkv, D]
+ *   (strides of token and head), each sequence's own k, v [B, T, Hkv, D] with lens[b] tokens in use
+ *   (clamped to 0..T), its Lq newest the queries': query i of sequence b sees the whole prefix and own
+ *   tokens 0 .. lens[b] - Lq + i.  Head h of q reads head h / (Hq / Hkv) of the keys.
+ *   out [B, Lq, Hq, D] = sum softmax(scale q k) v; 0 where a query sees no key.  weights (may be NULL)
+ *   [B, Hkv, T] fp32: the own tokens' softmax weights, summed over the Lq queries and the head's Hq / Hkv
+ *   query heads, are added to it.  dtype OTPU_BF16 or OTPU_F16 for q, caches and out; sums, maxima and
+ *   weights fp32.  D a multiple of 8, at most 256; scale > 0; addresses 16-byte aligned, strides
+ *   multiples of 8, tokens less than 2^22 elements apart.  P or T may be 0 (their operands NULL).
+ *   work: otpu_attn_work_bytes(...) bytes, 256-byte aligned, free again when the call's kernels ended. */
+int64_t otpu_attn_work_bytes(int B, int Lq, int Hq, int Hkv, int D, int P, int T);
+int otpu_attn_shared(const void* q, int64_t qb, int64_t qt, int64_t qh, const void* pk, int64_t pks,
+                     int64_t pkh, const void* pv, int64_t pvs, int64_t pvh, int P, const void* k, int64_t kb,
+                     int64_t kt, int64_t kh, const void* v, int64_t vb, int64_t vt, int64_t vh,
+                     const int32_t* lens, int T, int B, int Lq, int Hq, int Hkv, int D, int dtype, float scale,
+                     void* out, int64_t ob, int64_t ot, int64_t oh, float* weights, void* work,
+                     int64_t work_bytes, otpu_stream_t stream);
+
+/* Eviction from a cache by accumulated attention weight: where lens[b] > budget, each head keeps `budget`
+ * slots: those whose position is among the newest `recent` (pos > max pos - recent), then by weight, the
+ * lower slot where weights are equal (a NaN weight counts as the largest).  The j-th slot below budget
+ * that goes is overwritten by the j-th slot at or past budget that stays (rows of k and v in place, its
+ * weight and position); slots keep no order.  lens_out[b] = min(lens[b], budget); slots from there on get
+ * weight 0 and position -1.
+ *   k, v [B, T, H] rows of row_bytes bytes (a multiple of 16; strides kb, kt, kh, vb, vt, vh in bytes,
+ *   multiples of 16); weights fp32 and pos int32 [B, H, T]; weights_out, pos_out and lens_out are the old
+ *   arrays or ones that overlap nothing.  work: otpu_kv_evict_work_bytes(...) bytes, 256-byte aligned. */
+int64_t otpu_kv_evict_work_bytes(int B, int T, int H, int budget);
+int otpu_kv_evict(void* k, int64_t kb, int64_t kt, int64_t kh, void* v, int64_t vb, int64_t vt, int64_t vh,
+                  int row_bytes, const float* weights, const int32_t* pos, const int32_t* lens, int B, int T,
+                  int H, int budget, int recent, float* weights_out, int32_t* pos_out, int32_t* lens_out,
+                  void* work, int64_t work_bytes, otpu_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -18,6 +18,7 @@ FMT = {"int8": INT8, "int4": INT4, "fp4": FP4, "nvfp4": NVFP4}
 UNIT, ACC, RMAX, ASCALE, PAIR, RSC = 0x1, 0x2, 0x4, 0x8, 0x40, 0x80
 Q_ROW, Q_LO, Q_HL = 0x1, 0x10, 0x20             # QACT / QST flags
 ACT_ANY, ACT_ROW, ACT_MX = 0, 1, 2              # otpu_mm_dot: what is known of the activation offsets
+F32, BF16, F16 = 0, 1, 2                        # types of rows and caches (otpu_norm_qact, otpu_attn_shared)
 QALIGN = 64                                     # QACT ST / LDA row alignment
 LM_STATE_BYTES = 16640                          # the LM head's state (result word, maxima)
 ABI_VERSION = 3                                 # include/otpu.h OTPU_ABI_VERSION this binding follows
@@ -62,6 +63,13 @@ SIGNATURES = {
     "otpu_fake_act_f64": ([_P, _I, _I, _L, _I, _I, _I, _P, _L, _P, _L, _P], _I),
     "otpu_dequant": ([_P, _L, _P, _L, _I, _I, _I, _I, _P, _L, _P, _L, _P], _I),
     "otpu_mx_matmul": ([_P, _L, _P, _L, _P, _L, _P, _L, _I, _I, _I, _I, _I, _P, _L, _P], _I),
+    "otpu_norm_qact": ([_P, _L, _P, _L, _I, _I, _I, _P, _F, _I, _P, _L, _P, _P, _L, _P, _P, _L, _P], _I),
+    "otpu_attn_work_bytes": ([_I, _I, _I, _I, _I, _I, _I], _L),
+    "otpu_attn_shared": ([_P, _L, _L, _L, _P, _L, _L, _P, _L, _L, _I, _P, _L, _L, _L, _P, _L, _L, _L, _P, _I, _I, _I,
+                          _I, _I, _I, _I, _F, _P, _L, _L, _L, _P, _P, _L, _P], _I),
+    "otpu_kv_evict_work_bytes": ([_I, _I, _I, _I], _L),
+    "otpu_kv_evict": ([_P, _L, _L, _L, _P, _L, _L, _L, _I, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _L, _P],
+                      _I),
 }
 
 

@@ -202,6 +202,46 @@ def quantize_ranges(x, ranges=None, row_mode: bool = False):
     return _operand(q, Sa, da, ranges, bool(row_mode))
 
 
+NORM_TYPES = {}                                           # torch dtype -> the ABI's type, once torch is loaded
+
+
+def norm_quantize(x, gamma, residual=None, *, eps: float = 1e-6, row_mode: bool = False, h=None, r=None):
+    """The root-mean-square norm in front of a linear, with the residual's addition and QACT in one launch:
+    h = x + residual (fp32), r = 1 / sqrt(mean(h^2) + eps) a row, and the operand of (h * r) * gamma for
+    `dot` (an offset a group of 32; row_mode: one): as `fp32.qact` of the fp32 h with rscale r and cscale
+    gamma.  x [M, K] float32, bfloat16 or float16, residual of its type (or None), gamma [K]; K a multiple
+    of 32 (a `dot` needs 128).  Returns (operand, h): h in x's type, x itself without a residual.
+    h: a tensor for the sum, x or residual among them; r: a float32 tensor [M] for the rows' factors."""
+    T = X.torch()
+    if not NORM_TYPES:
+        NORM_TYPES.update({T.float32: X.F32, T.bfloat16: X.BF16, T.float16: X.F16})
+    if X.is_numpy(x):
+        x = X.dev(x, np.float32)
+        residual = None if residual is None else X.dev(residual, np.float32)
+    dt = x.dtype
+    if dt not in NORM_TYPES or x.dim() != 2 or not x.is_cuda:
+        raise ValueError(f"norm_quantize: x is {dt} {list(x.shape)} on {x.device}, needs [M, K] in float32, bfloat16 or float16")
+    M, K = x.shape
+    g = gamma if isinstance(gamma, T.Tensor) and gamma.dtype == T.float32 and gamma.is_contiguous() else X.dev(gamma, np.float32)
+    if g.shape != (K,):
+        raise ValueError(f"norm_quantize: gamma {list(g.shape)} over {K} columns")
+    if h is None and residual is not None:
+        h = T.empty((M, K), dtype=dt, device=x.device)
+    for name, t in (("x", x), ("residual", residual), ("h", h)):
+        if t is not None and (t.dtype != dt or t.shape != x.shape or t.device != x.device or (K > 1 and t.stride(1) != 1)):
+            raise ValueError(f"norm_quantize: {name} is {t.dtype} {list(t.shape)} on {t.device}, needs {dt} {[M, K]} on "
+                             f"{x.device}, columns adjacent")
+    if r is not None and (r.dtype != T.float32 or r.shape != (M,) or not r.is_contiguous() or r.device != x.device):
+        raise ValueError("norm_quantize: r is a contiguous float32 tensor [M]")
+    q = T.empty((M, K), dtype=T.int8, device=x.device)
+    d = T.empty((M, K // 32), dtype=T.uint8, device=x.device)
+    S = T.empty((1, M), dtype=T.float32, device=x.device)
+    X.call("otpu_norm_qact", x.data_ptr(), x.stride(0), X.ptr(residual), 0 if residual is None else residual.stride(0),
+           NORM_TYPES[dt], M, K, g.data_ptr(), eps, X.Q_ROW if row_mode else 0, X.ptr(h), 0 if h is None else h.stride(0),
+           X.ptr(r), q.data_ptr(), K, S.data_ptr(), d.data_ptr(), K // 32, X.stream())
+    return _operand(q, S, d, [K], bool(row_mode)), x if h is None else h
+
+
 def C_ptr(t, off: int):
     import ctypes
     return ctypes.c_void_p(t.data_ptr() + off * t.element_size())
@@ -414,5 +454,5 @@ def greedy(x, w: QWeight, chunk: int | None = None) -> int:
     return g.token()
 
 
-__all__ = ["mm", "mm_acc", "mm_spl", "lm_head_argmax", "argmax", "QWeight", "quantize_ranges", "dot", "Greedy",
+__all__ = ["mm", "mm_acc", "mm_spl", "lm_head_argmax", "argmax", "QWeight", "quantize_ranges", "norm_quantize", "dot", "Greedy",
            "greedy", "UNIT", "ACC", "RMAX", "ASCALE", "RSC", "WINDOW"]
