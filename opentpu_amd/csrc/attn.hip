@@ -4,8 +4,9 @@
 // multiplied once by the rows of every sequence together and each sequence's cache by its own rows.
 //
 //   segment_kernel   one segment's share of the keys for a tile of rows: partial o, m, l
-//   combine_kernel   the partials of a row joined, rounded to the output's type; the row's lse
-//   weights_kernel   the own keys' weights from the finished lse, added to the running sums
+//   combine_kernel   the partials of a row joined and rounded to the output's type; the own tokens'
+//                    weights from their scores
+//   weights_kernel   the weights where many rows would make the scores large: from the keys again
 #include "otpu_common.h"
 
 namespace otpu {
@@ -49,11 +50,15 @@ struct AttnArgs {
     float* weights;                          // [B, Hkv, T] or NULL
     int P, T, B, Lq, Hq, Hkv, G, D;
     float scale2;                            // scale * log2(e)
-    int sp, ss;                              // splits of the prefix, of the own keys
+    int sp, ss, per_p;                       // splits of the prefix, of the own keys; keys of a prefix split
+    uint32_t np, no;                         // workgroups of the prefix, of the own keys
+    bool keys_p, keys_o;                     // their shape
     float* po;                               // partial o [sp + ss][rows][D]
     float* pm;                               // m [sp + ss][rows]
     float* pl;                               // l [sp + ss][rows]
-    float* lse;                              // [rows]: log2 of the softmax's sum
+    float* lse;                              // [rows]: log2 of the softmax's sum, or NULL
+    float* sc;                               // own scores [B, Hkv, R][tp], or NULL
+    int64_t tp;
 };
 
 __device__ __forceinline__ uint32_t lds_addr(const void* p) {
@@ -64,7 +69,9 @@ __device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t l
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                  : : "v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory");
 }
-__device__ __forceinline__ void wait_all_dma() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+// wait until at most N of this wave's loads are outstanding
+template <int N>
+__device__ __forceinline__ void wait_dma() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory"); }
 __device__ __forceinline__ void bar() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
 
 __device__ __forceinline__ float swap32_max(float v) {
@@ -76,20 +83,22 @@ __device__ __forceinline__ float swap32_sum(float v) {
     return bitsf(p[0]) + bitsf(p[1]);
 }
 
-// A workgroup's shape: WR waves of 32 rows each times WK shares of the keys, KT keys a wave a step.
-template <int DP_, int WR_, int WK_, int KT_>
-struct Shape {
-    static constexpr int DP = DP_, WR = WR_, WK = WK_, KT = KT_;
-    static constexpr int NW = WR * WK;                     // waves
-    static constexpr int BM = WR * 32;                     // rows
-    static constexpr int NKEY = WK * KT;                   // keys a step
+// Two shapes of a workgroup of four waves:
+//   rows   128 rows, 32 a wave, against the same keys: KT keys and values a step through LDS, two stages
+//   keys   32 rows (or fewer) against keys that every wave takes 32 at a time for itself, without a barrier:
+//          its keys' next load is under way during the softmax and its values' product, its values' during
+//          the next scores
+// `keys` is bound by the loads of its keys whatever its rows, so 32 or fewer rows take it.
+constexpr int NW = 4;
+template <int DP_> struct Shape {
+    static constexpr int DP = DP_;
     static constexpr int CR = DP / 8;                      // 16-byte chunks a key
-    static constexpr int KB = NKEY * DP * 2;               // bytes of a step's keys (and of its values)
-    static constexpr int STAGE = 2 * KB;
-    static constexpr int LOADS = KB / 1024 / NW;           // direct loads a wave issues for the keys
-    static constexpr int MERGE = (WK - 1) * WR * 64 * (DP / 2 + 2) * 4;
-    static constexpr int LDS = 2 * STAGE > MERGE ? 2 * STAGE : MERGE;
-    static_assert(KB % (1024 * NW) == 0, "whole direct loads");
+    static constexpr int KT = DP <= 128 ? 64 : 32;         // rows: keys a step
+    static constexpr int RB = KT * DP * 2;                 // ... their bytes, and their values'
+    static constexpr int KB = 32 * DP * 2;                 // keys: a wave's keys' bytes, and its values'
+    static constexpr int MERGE = (NW - 1) * 64 * (DP / 2 + 2) * 4;
+    static constexpr int ROWS_LDS = 4 * RB, KEYS_LDS = NW * 2 * KB > MERGE ? NW * 2 * KB : MERGE;
+    static constexpr int LDS = ROWS_LDS > KEYS_LDS ? ROWS_LDS : KEYS_LDS;
 };
 
 // chunk c of key row r lies in slot c ^ f(r): the 8 (16) rows that lanes read together at one c on
@@ -97,309 +106,509 @@ struct Shape {
 template <int CR> __device__ __forceinline__ int kswz(int r) { return r & (CR < 16 ? CR - 1 : 15); }
 template <int CR> __device__ __forceinline__ int vswz(int r) { return (2 * r) & (CR < 16 ? CR - 1 : 15); }
 
-// The rows of a tile against keys [key0, key1) of a segment; lim: how many of the segment's keys this
-// lane's row sees.
-template <class E, class S, bool FULL, bool OWN>
-__device__ __forceinline__ void segment_tile(const AttnArgs& a, char* lds, const char* kbase, int64_t kstride,
-                                             const char* vbase, int64_t vstride, int key0, int key1, int lim,
-                                             const char* qrow, bool valid, int slot, int64_t row) {
-    constexpr int DP = S::DP, KT = S::KT, CR = S::CR, KS = DP / 16, DT = DP / 32, TT = KT / 32;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wr = wave % S::WR, wk = wave / S::WR;
-    const int r32 = lane & 31, hh = lane >> 5;
-    const int64_t rows = (int64_t)a.B * a.Lq * a.Hq;
-    float* const pm = a.pm + slot * rows + row;
-    float* const pl = a.pl + slot * rows + row;
-
-    const int n = key1 - key0;
-    if (n <= 0) {                                          // (uniform over the workgroup)
-        if (wk == 0 && valid && hh == 0) { *pm = -__builtin_inff(); *pl = 0.f; }
-        return;
-    }
-    if constexpr (!FULL) {                                 // columns past D: zeros that no load overwrites
-        for (int i = threadIdx.x; i < 2 * S::STAGE / 16; i += S::NW * 64)
-            reinterpret_cast<v4u*>(lds)[i] = v4u{0, 0, 0, 0};
-        bar();
-    }
-    // the row's query: B operand of K Q^T
-    v8s qf[KS];
+// Direct loads of `rows` rows of a segment from row r0 on into LDS at `to`, dealt to nw waves of which
+// this is number w; rows past `last` read it instead.
+template <int CR, bool FULL, bool VAL, int ROWS, int W>
+__device__ __forceinline__ void load_rows(const char* base, int64_t stride, int64_t r0, int last, uint32_t to, int w, int D) {
+    constexpr int RPL = 64 / CR, LOADS = ROWS / RPL / W;   // rows a load covers, loads a wave issues
+    const int lane = threadIdx.x & 63;
+    const uint64_t b64 = (uint64_t)(base + r0 * stride);   // (uniform: into scalar registers)
+    const char* const b = (const char*)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)b64) |
+                                        (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b64 >> 32)) << 32);
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
+    for (int u = 0; u < LOADS; ++u) {
+        const int r = (w * LOADS + u) * RPL + lane / CR;
+        const int c = (lane % CR) ^ (VAL ? vswz<CR>(r) : kswz<CR>(r));
+        if (FULL || c * 8 < D)
+            dma16(b, (uint32_t)min(r, last) * (uint32_t)stride + 16u * c, to + (uint32_t)(w * LOADS + u) * 1024u);
+    }
+}
+
+// what a wave holds of its 32 rows: lane (r32, hh) the row r32, of o^T the columns 8 r + 4 hh + 0..3 of
+// each 32, and half of the keys of l
+template <int DP> struct Acc {
+    v16f o[DP / 32];
+    float m, l;
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
+        m = -__builtin_inff();
+        l = 0.f;
+    }
+};
+
+// An infinity or NaN among the values of a key that some row does not see would reach that row as
+// 0 * inf.  So a step with such keys multiplies the finite values alone (the others are set to zero, and
+// the flag), and add_infinite adds the others to the partials of the rows that see them.
+template <class E>
+__device__ __forceinline__ void finite_values(char* vs, int pieces, int* flag) {
+    constexpr uint32_t EX = E::INF * 0x10001u, LO = (0x8000u - E::INF) * 0x10001u;
+#pragma unroll 1
+    for (int x = threadIdx.x & 63; x < pieces; x += 64) {
+        v4u w = reinterpret_cast<const v4u*>(vs)[x];
+        const v4u bad = ((w & EX) + LO) & 0x80008000u;     // bit 15 of each value that is not finite
+        if ((bad[0] | bad[1] | bad[2] | bad[3]) != 0) {
+            w &= ~((bad >> 15) * 0xFFFFu);
+            reinterpret_cast<v4u*>(vs)[x] = w;
+            *flag = 1;
+        }
+    }
+}
+
+// One step: 32 TT keys at ks and their values at vs (LDS) from the segment's key `at` on.  lim: the
+// segment's keys that this lane's row sees; first: the least of the wave's, least: of the workgroup's.
+// keys_read() runs once the keys are read, values_come() before the values are.  sc: the scores' row (or
+// NULL), for the weights.
+template <class E, int DP, int TT, bool OWN, class FK, class FV>
+__device__ __forceinline__ void step(Acc<DP>& a, const char* ks, const char* vs, int at, int lim, int first,
+                                     int least, int* flag, const v8s (&qf)[DP / 16], float c2, float* sc, FK keys_read,
+                                     FV values_come) {
+    constexpr int CR = DP / 8, KS = DP / 16, DT = DP / 32;
+    const int lane = threadIdx.x & 63, r32 = lane & 31, hh = lane >> 5;
+    v16f s[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
+        const int kr = t * 32 + r32;
+#pragma unroll
+        for (int x = 0; x < KS; ++x) {
+            const v8s kf = *reinterpret_cast<const v8s*>(ks + kr * (DP * 2) + (((2 * x + hh) ^ kswz<CR>(kr)) << 4));
+            s[t] = E::mma(kf, qf[x], s[t]);
+        }
+    }
+    keys_read();
+    if (OWN && sc) {
+#pragma unroll
+        for (int t = 0; t < TT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                *reinterpret_cast<v4f*>(sc + at + t * 32 + 8 * r + 4 * hh) =
+                    v4f{s[t][4 * r], s[t][4 * r + 1], s[t][4 * r + 2], s[t][4 * r + 3]};
+    }
+    const bool masked = at + 32 * TT > first;              // (uniform) keys that a row does not see
+    if (masked) {
+#pragma unroll
+        for (int t = 0; t < TT; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (at + t * 32 + 8 * (r / 4) + 4 * hh + r % 4 >= lim) s[t][r] = -__builtin_inff();
+    }
+    float mt = s[0][0];
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[t][r]);
+    mt = swap32_max(mt) * c2;
+    // the maximum is raised, and o and l scaled, only where a score passes it by more than 2^8: the
+    // weights stay below 2^8, exact in the same relative terms
+    if (__any(mt > a.m + 8.f)) {
+        const float mn = fmaxf(a.m, mt);
+        const float al = mn > -__builtin_inff() ? __builtin_amdgcn_exp2f(a.m - mn) : 1.f;
+        a.m = mn;
+        a.l *= al;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) a.o[t][r] *= al;
+    }
+    const float mu = a.m > -__builtin_inff() ? a.m : 0.f;  // (a row that has seen no key yet)
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], c2, -mu));
+            a.l += s[t][r];
+        }
+    values_come();
+    // o^T += V^T P^T: registers 8j .. 8j+7 of a score tile are this lane's keys 16j + 4 hh + 0..3
+    // and 16j + 8 + 4 hh + 0..3, the order in which the values' transposing reads give them
+    auto values = [&](int t, int j, int d) INL {
+        typedef __attribute__((address_space(3))) v4s lv4s;
+        const int kr = t * 32 + 16 * j + 4 * hh + (lane & 15) / 4;
+        const int c = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+        const char* const p0 = vs + kr * (DP * 2) + ((c ^ vswz<CR>(kr)) << 4) + 8 * (lane & 1);
+        const char* const p1 = vs + (kr + 8) * (DP * 2) + ((c ^ vswz<CR>(kr + 8)) << 4) + 8 * (lane & 1);
+        const v4s a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s*)p0);
+        const v4s a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s*)p1);
+        return __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    if (OWN && at + 32 * TT > least) finite_values<E>(const_cast<char*>(vs), 32 * TT * CR, flag);
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            typename E::v8 p;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[e] = (typename E::e)s[t][8 * j + e];
+            const v8s pb = __builtin_bit_cast(v8s, p);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) a.o[d] = E::mma(values(t, j, d), pb, a.o[d]);
+        }
+}
+
+// One workgroup's part: keys [key0, key1) of a segment for a tile of rows.
+struct Part {
+    const char *k, *v;                       // the segment's key 0 of the head
+    int64_t ks, vs;                          // byte strides of a token
+    int key0, key1, lim;                     // lim: the segment's keys that this lane's row sees
+    int least;                               // the least of the workgroup's rows
+    const char* q;                           // this lane's row
+    bool valid;                              // a row of its own (not the clamped last one)
+    int64_t at;                              // its place among the partials: (slot, row)
+    float* sc;                               // its scores' row, or NULL
+};
+
+template <int DP, bool FULL>
+__device__ __forceinline__ void load_query(v8s (&qf)[DP / 16], const char* q, int D) {
+    const int hh = (threadIdx.x >> 5) & 1;
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {                    // B operand of K Q^T
         const int c = 2 * s + hh;
-        if (FULL || c * 8 < a.D) qf[s] = *reinterpret_cast<const v8s*>(qrow + c * 16);
+        if (FULL || c * 8 < D) qf[s] = *reinterpret_cast<const v8s*>(q + c * 16);
         else qf[s] = v8s{0, 0, 0, 0, 0, 0, 0, 0};
     }
-    const uint32_t lds0 = lds_addr(lds);
-    const int steps = (n + S::NKEY - 1) / S::NKEY;
-    constexpr int RPL = 64 / CR;                           // key rows a direct load covers
-    auto issue = [&](int i) INL {
-        const char* kb = kbase + (int64_t)(key0 + i * S::NKEY) * kstride;
-        const char* vb = vbase + (int64_t)(key0 + i * S::NKEY) * vstride;
-        const uint32_t at = lds0 + (uint32_t)(i & 1) * S::STAGE;
-        const int last = n - 1 - i * S::NKEY;              // rows past the segment's end: its last key
-#pragma unroll
-        for (int u = 0; u < S::LOADS; ++u) {
-            const int r = (wave * S::LOADS + u) * RPL + lane / CR, sl = lane % CR;
-            const int rr = min(r, last);
-            const int ck = sl ^ kswz<CR>(r), cv = sl ^ vswz<CR>(r);
-            const uint32_t to = (uint32_t)(wave * S::LOADS + u) * 1024u;
-            if (FULL || ck * 8 < a.D) dma16(kb, (uint32_t)rr * (uint32_t)kstride + 16u * ck, at + to);
-            if (FULL || cv * 8 < a.D) dma16(vb, (uint32_t)rr * (uint32_t)vstride + 16u * cv, at + S::KB + to);
-        }
-    };
-    issue(0);
+}
 
-    v16f o[DT];
+template <int DP, bool FULL>
+__device__ __forceinline__ void store_part(const AttnArgs& a, const Acc<DP>& c, float l, const Part& p) {
+    if (!p.valid) return;
+    const int hh = (threadIdx.x >> 5) & 1;
+    if (hh == 0) { a.pm[p.at] = c.m; a.pl[p.at] = l; }
+    float* const po = a.po + p.at * a.D;
 #pragma unroll
-    for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
-    float m = -__builtin_inff(), l = 0.f;
-    const float c2 = a.scale2;
-    // the first key that some row of this wave does not see
-    int first = lim;
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) first = min(first, __shfl_xor(first, x, 64));
-    first = __builtin_amdgcn_readfirstlane(first);
-
-    for (int i = 0; i < steps; ++i) {
-        wait_all_dma();
-        bar();
-        if (i + 1 < steps) issue(i + 1);
-        const char* const ks = lds + (i & 1) * S::STAGE;
-        const char* const vs = ks + S::KB;
-        const int at = key0 + i * S::NKEY + wk * KT;       // the wave's first key
-        if (at >= key1) continue;
-
-        v16f s[TT];
-#pragma unroll
-        for (int t = 0; t < TT; ++t) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
-            const int kr = wk * KT + t * 32 + r32;
-            const char* const krow = ks + kr * (DP * 2);
-#pragma unroll
-            for (int x = 0; x < KS; ++x) {
-                const v8s kf = *reinterpret_cast<const v8s*>(krow + (((2 * x + hh) ^ kswz<CR>(kr)) << 4));
-                s[t] = E::mma(kf, qf[x], s[t]);
-            }
-        }
-        const bool masked = at + KT > first;               // (uniform) keys that a row does not see
-        if (masked) {
-#pragma unroll
-            for (int t = 0; t < TT; ++t)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (at + t * 32 + 8 * (r / 4) + 4 * hh + r % 4 >= lim) s[t][r] = -__builtin_inff();
-        }
-        float mt = s[0][0];
-#pragma unroll
-        for (int t = 0; t < TT; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[t][r]);
-        mt = swap32_max(mt) * c2;
-        // the maximum is raised, and o and l scaled, only where a score passes it by more than 2^8: the
-        // weights stay below 2^8, exact in the same relative terms
-        if (__any(mt > m + 8.f)) {
-            const float mn = fmaxf(m, mt);
-            const float al = mn > -__builtin_inff() ? __builtin_amdgcn_exp2f(m - mn) : 1.f;
-            m = mn;
-            l *= al;
-#pragma unroll
-            for (int t = 0; t < DT; ++t)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[t][r] *= al;
-        }
-        const float mu = m > -__builtin_inff() ? m : 0.f;  // (a row that has seen no key yet)
-#pragma unroll
-        for (int t = 0; t < TT; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], c2, -mu));
-                l += s[t][r];
-            }
-        // o^T += V^T P^T: registers 8j .. 8j+7 of a score tile are this lane's keys 16j + 4 hh + 0..3
-        // and 16j + 8 + 4 hh + 0..3, the order in which the values' transposing reads give them
-        auto values = [&](int t, int j, int d) INL {
-            typedef __attribute__((address_space(3))) v4s lv4s;
-            const int kr = wk * KT + t * 32 + 16 * j + 4 * hh + (lane & 15) / 4;
-            const int c = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-            const char* const p0 = vs + kr * (DP * 2) + ((c ^ vswz<CR>(kr)) << 4) + 8 * (lane & 1);
-            const char* const p1 = vs + (kr + 8) * (DP * 2) + ((c ^ vswz<CR>(kr + 8)) << 4) + 8 * (lane & 1);
-            const v4s a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s*)p0);
-            const v4s a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s*)p1);
-            return __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
-        };
-        if (OWN && masked) {
-            // an infinity or NaN among the values of a key that some row does not see would reach that
-            // row as 0 * inf: such a step multiplies the finite values alone, and then adds the others to
-            // the rows that see them
-            uint32_t bad = 0;
-            constexpr uint32_t EX = E::INF * 0x10001u, LO = (0x8000u - E::INF) * 0x10001u;
-#pragma unroll 1
-            for (int x = lane; x < KT * CR; x += 64) {
-                const v4u w = reinterpret_cast<const v4u*>(vs + wk * KT * (DP * 2))[x];
-                bad |= ((w[0] & EX) + LO) | ((w[1] & EX) + LO) | ((w[2] & EX) + LO) | ((w[3] & EX) + LO);
-            }
-            if (__any((bad & 0x80008000u) != 0)) {
-#pragma unroll 1
-                for (int kind = 0; kind < 4; ++kind) {     // finite, inf, -inf, NaN
-                    const float add = kind == 1 ? __builtin_inff() : (kind == 2 ? -__builtin_inff() : __builtin_nanf(""));
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) {
-                        __builtin_amdgcn_sched_barrier(0); // (not all columns at once: registers)
-                        v16f c;
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) c[r] = kind == 0 ? o[d][r] : 0.f;
-#pragma unroll
-                        for (int t = 0; t < TT; ++t)
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                v8s va = values(t, j, d);
-                                typename E::v8 p;
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) {
-                                    const int key = at + t * 32 + 16 * j + 8 * (e / 4) + 4 * hh + e % 4;
-                                    p[e] = (typename E::e)(kind == 0 ? s[t][8 * j + e] : (key < lim ? 1.f : 0.f));
-                                    const uint16_t x = (uint16_t)va[e];
-                                    const int is = (x & 0x7FFF) < E::INF ? 0 : ((x & 0x7FFF) > E::INF ? 3 : (x >> 15) + 1);
-                                    va[e] = (short)(kind == is ? (kind == 0 ? x : E::ONE) : 0);
-                                }
-                                c = E::mma(va, __builtin_bit_cast(v8s, p), c);
-                            }
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) o[d][r] = kind == 0 ? c[r] : (c[r] > 0.f ? o[d][r] + add : o[d][r]);
-                    }
-                }
-                continue;
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < TT; ++t)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                typename E::v8 p;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) p[e] = (typename E::e)s[t][8 * j + e];
-                const v8s pb = __builtin_bit_cast(v8s, p);
-#pragma unroll
-                for (int d = 0; d < DT; ++d) o[d] = E::mma(values(t, j, d), pb, o[d]);
-            }
-    }
-    l = swap32_sum(l);
-
-    // the key shares of a row tile joined through LDS (o and l relative to a common m)
-    if constexpr (S::WK > 1) {
-        constexpr int ST = DP / 2 + 2;
-        float* const x = reinterpret_cast<float*>(lds);
-        bar();
-        if (wk > 0) {
-            float* const y = x + (((wk - 1) * S::WR + wr) * ST) * 64 + lane;
-#pragma unroll
-            for (int t = 0; t < DT; ++t)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) y[(t * 16 + r) * 64] = o[t][r];
-            y[(DP / 2) * 64] = m;
-            y[(DP / 2 + 1) * 64] = l;
-        }
-        bar();
-        if (wk > 0) return;
-#pragma unroll
-        for (int w = 1; w < S::WK; ++w) {
-            const float* const y = x + (((w - 1) * S::WR + wr) * ST) * 64 + lane;
-            const float m1 = y[(DP / 2) * 64], mn = fmaxf(m, m1);
-            const float e0 = m > -__builtin_inff() ? __builtin_amdgcn_exp2f(m - mn) : 0.f;
-            const float e1 = m1 > -__builtin_inff() ? __builtin_amdgcn_exp2f(m1 - mn) : 0.f;
-            l = l * e0 + y[(DP / 2 + 1) * 64] * e1;
-            m = mn;
-#pragma unroll
-            for (int t = 0; t < DT; ++t)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[t][r] = o[t][r] * e0 + y[(t * 16 + r) * 64] * e1;
-        }
-    }
-    if (!valid) return;
-    if (hh == 0) { *pm = m; *pl = l; }
-    float* const po = a.po + (slot * rows + row) * a.D;
-#pragma unroll
-    for (int t = 0; t < DT; ++t)
+    for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int d = t * 32 + 8 * r + 4 * hh;
             if (FULL || d < a.D)
-                *reinterpret_cast<v4f*>(po + d) = v4f{o[t][4 * r], o[t][4 * r + 1], o[t][4 * r + 2], o[t][4 * r + 3]};
+                *reinterpret_cast<v4f*>(po + d) = v4f{c.o[t][4 * r], c.o[t][4 * r + 1], c.o[t][4 * r + 2], c.o[t][4 * r + 3]};
         }
 }
 
-// Prefix: workgroup (head, row tile, split), the heads spread over the XCDs and a split's row tiles next
-// to each other, so that one L2 serves them the same keys.  Own: workgroup (sequence, head, row tile,
-// split).
-template <class E, class S, bool FULL, bool OWN>
-__global__ __launch_bounds__(S::NW * 64) void segment_kernel(AttnArgs a, int tiles) {
-    __shared__ __attribute__((aligned(16))) char lds[S::LDS];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int R = a.Lq * a.G;
-    const int h = blockIdx.x % a.Hkv;
-    int x = blockIdx.x / a.Hkv;
-    const int tile = x % tiles;
-    x /= tiles;
-    const int mrow = tile * S::BM + (wave % S::WR) * 32 + (lane & 31);
-    if constexpr (!OWN) {
-        const int M = a.B * R, split = x;
-        const int mc = min(mrow, M - 1);
-        const int b = mc / R, rem = mc - b * R, i = rem / a.G, g = rem - i * a.G;
-        const int head = h * a.G + g;
-        const int per = (((a.P + a.sp - 1) / a.sp) + 63) & ~63;
-        const int key0 = min(split * per, a.P), key1 = min(key0 + per, a.P);
-        segment_tile<E, S, FULL, OWN>(a, lds, a.pk + h * a.pkh, a.pks, a.pv + h * a.pvh, a.pvs, key0, key1, key1,
-                                 a.q + b * a.qb + i * a.qt + head * a.qh, mrow < M, split,
-                                 ((int64_t)b * a.Lq + i) * a.Hq + head);
-    } else {
-        const int b = x / a.ss, split = x % a.ss;
-        const int len = min(max(a.lens[b], 0), a.T);
-        const int mc = min(mrow, R - 1);
-        const int i = mc / a.G, g = mc - i * a.G, head = h * a.G + g;
-        const int ilast = min((tile + 1) * S::BM, R) - 1;
-        const int seen = max(len - a.Lq + ilast / a.G + 1, 0);          // keys that the tile's last row sees
-        const int per = (((seen + a.ss - 1) / a.ss) + 63) & ~63;
-        const int key0 = min(split * per, seen), key1 = min(key0 + per, seen);
-        segment_tile<E, S, FULL, OWN>(a, lds, a.k + b * a.kb + h * a.kh, a.kt, a.v + b * a.vb + h * a.vh, a.vt, key0, key1,
-                                 min(len - a.Lq + i + 1, key1), a.q + b * a.qb + i * a.qt + head * a.qh, mrow < R,
-                                 a.sp + split, ((int64_t)b * a.Lq + i) * a.Hq + head);
+// the values that finite_values took out, from keys of tiles of KT, added to the partials of the wave's rows
+// that see them
+template <class E, int KT>
+__device__ __forceinline__ void add_infinite(const AttnArgs& a, const Part& p) {
+    const int lane = threadIdx.x & 63;
+    const int from = p.key0 + max(p.least - p.key0, 0) / KT * KT;
+    __threadfence();
+    for (int r = 0; r < 32; ++r) {
+        if (!__shfl((int)p.valid, r, 64)) continue;
+        const int lim = __shfl(p.lim, r, 64);
+        float* const po = a.po + __shfl(p.at, r, 64) * a.D;
+        for (int d = lane; d < a.D; d += 64) {
+            float add = 0.f;
+            for (int t = from; t < lim; ++t) {
+                const float x = (float)reinterpret_cast<const typename E::e*>(p.v + (int64_t)t * p.vs)[d];
+                if (!(__builtin_fabsf(x) < __builtin_inff())) add += x;
+            }
+            if (add != 0.f) po[d] += add;
+        }
     }
 }
 
-// a thread: four columns of a row, over the row's partials
-template <class E>
-__global__ __launch_bounds__(256) void combine_kernel(AttnArgs a) {
-    const int64_t rows = (int64_t)a.B * a.Lq * a.Hq;
-    const int per = a.D / 4;
-    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (t >= rows * per) return;
-    const int64_t row = t / per;
-    const int d = (int)(t - row * per) * 4;
-    const int n = a.sp + a.ss;
-    float m = -__builtin_inff();
-    for (int s = 0; s < n; ++s) m = fmaxf(m, a.pm[s * rows + row]);
-    float l = 0.f;
-    v4f o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < n; ++s) {
-        const float ms = a.pm[s * rows + row];
-        if (ms == -__builtin_inff()) continue;
-        const float w = __builtin_amdgcn_exp2f(ms - m);
-        l += w * a.pl[s * rows + row];
-        const v4f x = *reinterpret_cast<const v4f*>(a.po + (s * rows + row) * a.D + d);
-        o += w * x;
-    }
-    const float il = l == 0.f ? 0.f : 1.f / l;
-    typename E::v4 y;
+__device__ __forceinline__ int wave_min(int x) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = (typename E::e)(o[j] * il);
+    for (int o = 16; o > 0; o >>= 1) x = min(x, __shfl_xor(x, o, 64));   // (both halves hold the same rows)
+    return __builtin_amdgcn_readfirstlane(x);
+}
+
+// columns past D: zeros that no load overwrites
+__device__ __forceinline__ void clear_lds(char* lds, int bytes) {
+    for (int i = threadIdx.x; i < bytes / 16; i += NW * 64) reinterpret_cast<v4u*>(lds)[i] = v4u{0, 0, 0, 0};
+    bar();
+}
+
+template <class E, int DP, bool FULL, bool OWN>
+__device__ __forceinline__ void rows_part(const AttnArgs& a, char* lds, const Part& p) {
+    using S = Shape<DP>;
+    constexpr int KT = S::KT, CR = S::CR;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Acc<DP> c;
+    c.clear();
+    int* const flag = reinterpret_cast<int*>(lds + S::LDS);
+    if (OWN) *flag = 0;                                    // (every thread; a barrier follows)
+    if (!FULL) clear_lds(lds, S::ROWS_LDS);
+    v8s qf[DP / 16];
+    load_query<DP, FULL>(qf, p.q, a.D);
+    const uint32_t lds0 = lds_addr(lds);
+    const int n = p.key1 - p.key0, steps = (n + KT - 1) / KT;
+    auto issue = [&](int i) INL {
+        const uint32_t to = lds0 + (uint32_t)((i & 1) * 2 * S::RB);
+        load_rows<CR, FULL, false, KT, NW>(p.k, p.ks, p.key0 + i * KT, n - 1 - i * KT, to, wave, a.D);
+        load_rows<CR, FULL, true, KT, NW>(p.v, p.vs, p.key0 + i * KT, n - 1 - i * KT, to + S::RB, wave, a.D);
+    };
+    issue(0);
+    const int first = wave_min(p.lim), none = -wave_min(-p.lim);
+    for (int i = 0; i < steps; ++i) {
+        wait_dma<0>();
+        bar();
+        if (i + 1 < steps) issue(i + 1);
+        const char* const ks = lds + (i & 1) * 2 * S::RB;
+        const int at = p.key0 + i * KT;
+        if (OWN && at >= none) continue;                   // (uniform over the wave) no row of it sees these keys
+        step<E, DP, KT / 32, OWN>(c, ks, ks + S::RB, at, p.lim, first, p.least, flag, qf, a.scale2, nullptr, [] {}, [] {});
+    }
+    store_part<DP, FULL>(a, c, swap32_sum(c.l), p);
+    if constexpr (OWN) {
+        bar();
+        if (*flag) add_infinite<E, KT>(a, p);
+    }
+}
+
+template <class E, int DP, bool FULL, bool OWN>
+__device__ __forceinline__ void keys_part(const AttnArgs& a, char* lds, const Part& p) {
+    using S = Shape<DP>;
+    constexpr int CR = S::CR, LOADS = 32 / (64 / CR);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Acc<DP> c;
+    c.clear();
+    int* const flag = reinterpret_cast<int*>(lds + S::LDS);
+    if (OWN) { *flag = 0; bar(); }                         // (no other barrier before the last)
+    if (!FULL) clear_lds(lds, S::KEYS_LDS);
+    char* const ks = lds + wave * 2 * S::KB;
+    char* const vs = ks + S::KB;
+    const uint32_t kl = lds_addr(ks), vl = lds_addr(vs);
+    const int n = p.key1 - p.key0, tiles = (n + 31) / 32;
+    auto keys = [&](int j) INL { load_rows<CR, FULL, false, 32, 1>(p.k, p.ks, p.key0 + 32 * j, n - 1 - 32 * j, kl, 0, a.D); };
+    auto vals = [&](int j) INL { load_rows<CR, FULL, true, 32, 1>(p.v, p.vs, p.key0 + 32 * j, n - 1 - 32 * j, vl, 0, a.D); };
+    v8s qf[DP / 16];
+    load_query<DP, FULL>(qf, p.q, a.D);
+    const int first = wave_min(p.lim);
+    if (wave < tiles) { keys(wave); vals(wave); }
+    for (int j = wave; j < tiles; j += NW) {
+        const bool more = j + NW < tiles;
+        wait_dma<LOADS>();                                 // the keys are there; the values' loads are younger
+        step<E, DP, 1, OWN>(c, ks, vs, p.key0 + 32 * j, p.lim, first, p.least, flag, qf, a.scale2, p.sc,
+            [&]() INL {
+                asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+                if (more) keys(j + NW);
+            },
+            [&]() INL {
+                if (more) wait_dma<LOADS>();               // (the next keys' loads are younger)
+                else wait_dma<0>();
+            });
+        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+        if (more) vals(j + NW);
+    }
+    float l = swap32_sum(c.l);
+    // the waves' shares joined through LDS
+    constexpr int ST = DP / 2 + 2;
+    float* const x = reinterpret_cast<float*>(lds);
+    bar();
+    if (wave > 0) {
+        float* const y = x + (wave - 1) * ST * 64 + lane;
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) y[(t * 16 + r) * 64] = c.o[t][r];
+        y[(DP / 2) * 64] = c.m;
+        y[(DP / 2 + 1) * 64] = l;
+    }
+    bar();
+    if (wave > 0) return;
+    for (int w = 0; w < NW - 1 && w + 1 < tiles; ++w) {
+        const float* const y = x + w * ST * 64 + lane;
+        const float m1 = y[(DP / 2) * 64], mn = fmaxf(c.m, m1);
+        const float e0 = c.m > -__builtin_inff() ? __builtin_amdgcn_exp2f(c.m - mn) : 0.f;
+        const float e1 = m1 > -__builtin_inff() ? __builtin_amdgcn_exp2f(m1 - mn) : 0.f;
+        l = l * e0 + y[(DP / 2 + 1) * 64] * e1;
+        c.m = mn;
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) c.o[t][r] = c.o[t][r] * e0 + y[(t * 16 + r) * 64] * e1;
+    }
+    store_part<DP, FULL>(a, c, l, p);
+    if constexpr (OWN)
+        if (*flag) add_infinite<E, 32>(a, p);
+}
+
+// The workgroups of the prefix, then those of the own keys.  Prefix: (head, row tile, split), the heads over
+// the XCDs and a split's row tiles next to each other, so that one L2 serves them the same keys.  (Both
+// kinds in turn, for the products of the one beside the loads of the other, takes that sharing from the
+// row tiles: 256 sequences on 131072 tokens 743 us, one kind after the other 526.)  Own: (head, row tile,
+// sequence, split).
+template <class E, int DP, bool FULL>
+__global__ __launch_bounds__(NW * 64, DP <= 128 ? 2 : 1) void segment_kernel(AttnArgs a) {
+    __shared__ __attribute__((aligned(16))) char lds[Shape<DP>::LDS + 16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int R = a.Lq * a.G;
+    const int64_t rows = (int64_t)a.B * a.Lq * a.Hq;
+    const bool own = blockIdx.x >= a.np;
+    uint32_t x = own ? blockIdx.x - a.np : blockIdx.x;
+    const int h = x % a.Hkv;
+    x /= a.Hkv;
+    const bool keys = own ? a.keys_o : a.keys_p;
+    const int wrow = (keys ? 0 : wave * 32) + (lane & 31), bm = keys ? 32 : 32 * NW;
+    Part p;
+    if (!own) {
+        const int M = a.B * R, tiles = (M + bm - 1) / bm;
+        const int tile = x % tiles, split = x / tiles;
+        const int mrow = tile * bm + wrow, mc = min(mrow, M - 1);
+        const int b = mc / R, rem = mc - b * R, i = rem / a.G, head = h * a.G + rem - i * a.G;
+        p.key0 = min(split * a.per_p, a.P);
+        p.key1 = min(p.key0 + a.per_p, a.P);
+        p.lim = p.least = p.key1;
+        p.k = a.pk + h * a.pkh; p.ks = a.pks;
+        p.v = a.pv + h * a.pvh; p.vs = a.pvs;
+        p.q = a.q + b * a.qb + i * a.qt + head * a.qh;
+        p.valid = mrow < M;
+        p.at = split * rows + ((int64_t)b * a.Lq + i) * a.Hq + head;
+        p.sc = nullptr;
+    } else {
+        const int tiles = (R + bm - 1) / bm;
+        const int tile = x % tiles, b = x / tiles % a.B, split = x / tiles / a.B;
+        const int mrow = tile * bm + wrow, mc = min(mrow, R - 1);
+        const int i = mc / a.G, g = mc - i * a.G, head = h * a.G + g;
+        const int len = min(max(a.lens[b], 0), a.T);
+        const int seen = max(len - a.Lq + (min((tile + 1) * bm, R) - 1) / a.G + 1, 0);   // by the tile's last row
+        const int per = ((seen + a.ss - 1) / a.ss + 31) & ~31;
+        p.key0 = min(split * per, seen);
+        p.key1 = min(p.key0 + per, seen);
+        p.lim = min(len - a.Lq + i + 1, p.key1);
+        p.least = min(len - a.Lq + tile * bm / a.G + 1, p.key1);
+        p.k = a.k + b * a.kb + h * a.kh; p.ks = a.kt;
+        p.v = a.v + b * a.vb + h * a.vh; p.vs = a.vt;
+        p.q = a.q + b * a.qb + i * a.qt + head * a.qh;
+        p.valid = mrow < R;
+        p.at = (a.sp + split) * rows + ((int64_t)b * a.Lq + i) * a.Hq + head;
+        p.sc = a.sc && p.valid ? a.sc + (((int64_t)b * a.Hkv + h) * R + mc) * a.tp : nullptr;
+    }
+    if (p.key1 <= p.key0) {                                // (uniform over the workgroup)
+        if (p.valid && (keys ? wave == 0 : true) && lane < 32) { a.pm[p.at] = -__builtin_inff(); a.pl[p.at] = 0.f; }
+        return;
+    }
+    if (!own) {
+        if (keys) keys_part<E, DP, FULL, false>(a, lds, p);
+        else rows_part<E, DP, FULL, false>(a, lds, p);
+    } else {
+        if (keys) keys_part<E, DP, FULL, true>(a, lds, p);
+        else rows_part<E, DP, FULL, true>(a, lds, p);
+    }
+}
+
+// The partials of a row joined: GP threads take every GP-th partial of four columns, their sums meet in
+// LDS.  Workgroups past the rows' add the own tokens' weights from the scores: 1024 tokens of a (sequence,
+// head) each, the rows' sums joined again.
+constexpr int WT = 1024;
+template <class E, int GP>
+__global__ __launch_bounds__(256) void combine_kernel(AttnArgs a, int nrows) {
+    __shared__ float sm[256], sl[256];
+    __shared__ v4f so[256];
+    const int64_t rows = (int64_t)a.B * a.Lq * a.Hq;
+    const int n = a.sp + a.ss, tid = threadIdx.x;
+    if ((int)blockIdx.x >= nrows) {
+        const int R = a.Lq * a.G, nt = (a.T + WT - 1) / WT;
+        const int x = blockIdx.x - nrows, bh = x / nt, t0 = x % nt * WT;
+        const int b = bh / a.Hkv, h = bh - b * a.Hkv;
+        const int len = min(max(a.lens[b], 0), a.T);
+        if (t0 >= len) return;
+        // (R <= 32) a row's lse: 8 threads over its partials
+        {
+            const int r = min(tid >> 3, R - 1), i = r / a.G;
+            const int64_t row = ((int64_t)b * a.Lq + i) * a.Hq + h * a.G + r - i * a.G;
+            float m = -__builtin_inff(), l = 0.f;
+            for (int s = tid & 7; s < n; s += 8) {
+                const float m1 = a.pm[s * rows + row], l1 = a.pl[s * rows + row];
+                const float mn = fmaxf(m, m1);
+                if (mn > -__builtin_inff()) l = l * __builtin_amdgcn_exp2f(m - mn) + l1 * __builtin_amdgcn_exp2f(m1 - mn);
+                m = mn;
+            }
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) {
+                const float m1 = __shfl_xor(m, o, 64), l1 = __shfl_xor(l, o, 64), mn = fmaxf(m, m1);
+                if (mn > -__builtin_inff()) l = l * __builtin_amdgcn_exp2f(m - mn) + l1 * __builtin_amdgcn_exp2f(m1 - mn);
+                m = mn;
+            }
+            if ((tid & 7) == 0) sm[tid >> 3] = m + __builtin_log2f(l);
+        }
+        __syncthreads();
+        const int t = t0 + 4 * tid;
+        if (t >= len) return;
+        const float* const sc = a.sc + (int64_t)bh * R * a.tp + t;
+        v4f w = {0.f, 0.f, 0.f, 0.f};
+        for (int r = 0; r < R; ++r) {
+            const int see = len - a.Lq + r / a.G;           // the row's own token
+            const v4f s = *reinterpret_cast<const v4f*>(sc + (int64_t)r * a.tp);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (t + j <= see) w[j] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], a.scale2, -sm[r]));
+        }
+        float* const out = a.weights + (int64_t)bh * a.T + t;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (t + j < len) out[j] += w[j];
+        return;
+    }
+    const int per = a.D / 4, rpb = 256 / (per * GP);       // rows a workgroup
+    const int rl = tid / (per * GP), y = tid - rl * per * GP, g = y / per, d = (y - g * per) * 4;
+    const int64_t row = (int64_t)blockIdx.x * rpb + rl;
+    const bool ok = rl < rpb && row < rows;
+    float m = -__builtin_inff(), l = 0.f;
+    v4f o = {0.f, 0.f, 0.f, 0.f};
+    if (ok) {
+        constexpr int U = 4;                               // partials whose loads go out together
+        for (int s0 = g; s0 < n; s0 += U * GP) {
+            float ms[U], ls[U];
+            v4f os[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int s = s0 + u * GP;
+                ms[u] = -__builtin_inff();
+                ls[u] = 0.f;
+                if (s < n) {
+                    ms[u] = a.pm[s * rows + row];
+                    ls[u] = a.pl[s * rows + row];
+                    os[u] = *reinterpret_cast<const v4f*>(a.po + (s * rows + row) * a.D + d);
+                }
+            }
+            float mn = m;
+#pragma unroll
+            for (int u = 0; u < U; ++u) mn = fmaxf(mn, ms[u]);
+            if (mn == -__builtin_inff()) continue;
+            const float e = __builtin_amdgcn_exp2f(m - mn);
+            l *= e;
+            o *= e;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (ms[u] > -__builtin_inff()) {           // (a share without a key has no o)
+                    const float w = __builtin_amdgcn_exp2f(ms[u] - mn);
+                    l += w * ls[u];
+                    o += w * os[u];
+                }
+            m = mn;
+        }
+    }
+    if constexpr (GP > 1) {
+        sm[tid] = m;
+        sl[tid] = l;
+        so[tid] = o;
+        __syncthreads();
+        if (!ok || g > 0) return;
+#pragma unroll
+        for (int k = 1; k < GP; ++k) {
+            const float m1 = sm[tid + k * per];
+            if (m1 == -__builtin_inff()) continue;
+            const float mn = fmaxf(m, m1), e0 = __builtin_amdgcn_exp2f(m - mn), e1 = __builtin_amdgcn_exp2f(m1 - mn);
+            l = l * e0 + sl[tid + k * per] * e1;
+            o = o * e0 + so[tid + k * per] * e1;
+            m = mn;
+        }
+    }
+    if (!ok) return;
+    const float il = l == 0.f ? 0.f : 1.f / l;
+    typename E::v4 z;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) z[j] = (typename E::e)(o[j] * il);
     const int head = (int)(row % a.Hq);
     const int64_t bi = row / a.Hq;
     const int i = (int)(bi % a.Lq);
     const int64_t b = bi / a.Lq;
-    *reinterpret_cast<typename E::v4*>(a.out + b * a.ob + i * a.ot + head * a.oh + d * 2) = y;
+    *reinterpret_cast<typename E::v4*>(a.out + b * a.ob + i * a.ot + head * a.oh + d * 2) = z;
     if (a.lse && d == 0) a.lse[row] = m + __builtin_log2f(l);
 }
 
@@ -457,62 +666,67 @@ __global__ __launch_bounds__(256) void weights_kernel(AttnArgs a) {
 // ---- the host's side --------------------------------------------------------------------------
 
 struct Plan {
-    int bm_p, bm_o;                          // rows of a tile: prefix, own
-    int sp, ss;                              // splits
-    int64_t rows;
-    int64_t bytes;
+    bool keys_p, keys_o;                     // the workgroups' shape: prefix, own
+    int sp, ss, per_p;                       // splits; keys of a prefix split
+    int64_t np, no;                          // workgroups
+    int64_t rows, tp;
+    bool scores;                             // own scores kept for the weights
+    int64_t po, pm, pl, lse, sc, bytes;      // the work area's parts, in floats; its size
 };
 
-static int tile_rows(int rows) { return rows <= 32 ? 32 : (rows <= 64 ? 64 : 128); }
-
 static Plan plan(int B, int Lq, int Hq, int Hkv, int D, int P, int T) {
-    Plan p;
-    const int R = Lq * (Hq / Hkv), cu = otpu_cu_count();
-    const int64_t M = (int64_t)B * R;
+    Plan p = {};
+    const int R = Lq * (Hq / Hkv);
+    const int64_t M = (int64_t)B * R, slots = 2 * (int64_t)otpu_cu_count();
     p.rows = (int64_t)B * Lq * Hq;
-    p.bm_p = tile_rows((int)(M < 128 ? M : 128));
-    p.bm_o = tile_rows(R < 128 ? R : 128);
-    auto splits = [&](int64_t groups, int keys) {
+    p.keys_p = M <= 32;
+    p.keys_o = R <= 32;
+    const int64_t gp = (int64_t)Hkv * (p.keys_p ? 1 : (M + 127) / 128);
+    const int64_t go = (int64_t)B * Hkv * (p.keys_o ? 1 : (R + 127) / 128);
+    // as many splits as fill the CUs' places, of no fewer keys than pay for a partial
+    auto splits = [&](int64_t groups, int keys, int least) {
         if (keys <= 0 || groups <= 0) return 0;
-        int64_t s = (cu + groups - 1) / groups;
-        const int most = (keys + 255) / 256;
-        return (int)(s > most ? most : (s < 1 ? 1 : s));
+        const int64_t s = (slots + groups - 1) / groups, most = (keys + least - 1) / least;
+        return (int)(s > most ? most : s);
     };
-    p.sp = splits((int64_t)Hkv * ((M + p.bm_p - 1) / p.bm_p), P);
-    p.ss = splits((int64_t)B * Hkv * ((R + p.bm_o - 1) / p.bm_o), T);
+    p.sp = splits(gp, P, p.keys_p ? 128 : 512);
+    p.ss = splits(go, T, 256);
+    p.per_p = p.sp ? ((P + p.sp - 1) / p.sp + 31) & ~31 : 0;
+    p.np = gp * p.sp;
+    p.no = go * p.ss;
+    p.scores = p.keys_o;
+    p.tp = (T + 31) & ~31;
     const int64_t n = p.sp + p.ss;
-    p.bytes = 4 * (n * p.rows * (D + 2) + p.rows) + 256;
+    auto part = [&](int64_t floats) {
+        const int64_t at = p.bytes / 4;
+        p.bytes += (4 * floats + 255) & ~(int64_t)255;
+        return at;
+    };
+    p.po = part(n * p.rows * D);
+    p.pm = part(n * p.rows);
+    p.pl = part(n * p.rows);
+    p.lse = part(p.rows);
+    p.sc = part(p.scores ? (int64_t)B * Hkv * R * p.tp : 0);
     return p;
 }
 
-template <class E, class S, bool FULL>
-static void launch_segment(const AttnArgs& a, bool own, hipStream_t s) {
-    const int64_t m = own ? (int64_t)a.Lq * a.G : (int64_t)a.B * a.Lq * a.G;
-    const int tiles = (int)((m + S::BM - 1) / S::BM);
-    const int64_t grid = (int64_t)a.Hkv * tiles * (own ? (int64_t)a.B * a.ss : a.sp);
-    if (own) segment_kernel<E, S, FULL, true><<<(unsigned)grid, S::NW * 64, 0, s>>>(a, tiles);
-    else segment_kernel<E, S, FULL, false><<<(unsigned)grid, S::NW * 64, 0, s>>>(a, tiles);
-}
-
-template <class E, int DP, bool FULL>
-static void launch_bm(const AttnArgs& a, bool own, int bm, hipStream_t s) {
-    if constexpr (DP <= 128) {
-        if (bm == 32) launch_segment<E, Shape<DP, 1, 4, 32>, FULL>(a, own, s);
-        else if (bm == 64) launch_segment<E, Shape<DP, 2, 4, 32>, FULL>(a, own, s);
-        else launch_segment<E, Shape<DP, 4, 2, 64>, FULL>(a, own, s);
-    } else {
-        if (bm == 32) launch_segment<E, Shape<DP, 1, 2, 32>, FULL>(a, own, s);
-        else if (bm == 64) launch_segment<E, Shape<DP, 2, 2, 32>, FULL>(a, own, s);
-        else launch_segment<E, Shape<DP, 4, 1, 32>, FULL>(a, own, s);
-    }
+template <class E, int GP>
+static void launch_combine(const AttnArgs& a, const Plan& p, hipStream_t s) {
+    const int rpb = 256 / (a.D / 4 * GP);
+    const int nrows = (int)((p.rows + rpb - 1) / rpb);
+    const int nw = a.sc ? a.B * a.Hkv * ((a.T + WT - 1) / WT) : 0;
+    combine_kernel<E, GP><<<nrows + nw, 256, 0, s>>>(a, nrows);
 }
 
 template <class E, int DP, bool FULL>
 static void launch_all(const AttnArgs& a, const Plan& p, hipStream_t s) {
-    if (a.sp) launch_bm<E, DP, FULL>(a, false, p.bm_p, s);
-    if (a.ss) launch_bm<E, DP, FULL>(a, true, p.bm_o, s);
-    combine_kernel<E><<<(unsigned)((p.rows * (a.D / 4) + 255) / 256), 256, 0, s>>>(a);
-    if (a.weights && a.T)
+    if (p.np + p.no) segment_kernel<E, DP, FULL><<<(unsigned)(p.np + p.no), NW * 64, 0, s>>>(a);
+    // threads a partial's row: by how many partials there are (at most 256 in all: D / 4 columns' threads)
+    const int n = p.sp + p.ss;
+    if (n > 8 && a.D <= 128) launch_combine<E, 8>(a, p, s);
+    else if (n > 4) launch_combine<E, 4>(a, p, s);
+    else launch_combine<E, 1>(a, p, s);
+    if (a.weights && a.T && !a.sc)
         weights_kernel<E, DP, FULL><<<(unsigned)((int64_t)a.B * a.Hkv * ((a.T + 127) / 128)), 256, 0, s>>>(a);
 }
 
@@ -583,12 +797,16 @@ extern "C" int otpu_attn_shared(const void* q, int64_t qb, int64_t qt, int64_t q
     a.weights = weights;
     a.P = P; a.T = T; a.B = B; a.Lq = Lq; a.Hq = Hq; a.Hkv = Hkv; a.G = Hq / Hkv; a.D = D;
     a.scale2 = scale * 1.4426950408889634f;
-    a.sp = p.sp; a.ss = p.ss;
-    const int64_t n = p.sp + p.ss;
-    a.po = (float*)work;
-    a.pm = a.po + n * p.rows * D;
-    a.pl = a.pm + n * p.rows;
-    a.lse = a.pl + n * p.rows;
+    a.sp = p.sp; a.ss = p.ss; a.per_p = p.per_p;
+    a.np = (uint32_t)p.np; a.no = (uint32_t)p.no;
+    a.keys_p = p.keys_p; a.keys_o = p.keys_o;
+    float* const f = (float*)work;
+    a.po = f + p.po; a.pm = f + p.pm; a.pl = f + p.pl;
+    a.tp = p.tp;
+    if (weights && T) {
+        if (p.scores) a.sc = f + p.sc;
+        else a.lse = f + p.lse;
+    }
     const hipStream_t s = (hipStream_t)stream;
     if (dtype == OTPU_BF16) launch_type<BF16>(a, p, s);
     else launch_type<F16>(a, p, s);
