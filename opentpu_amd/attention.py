@@ -7,6 +7,8 @@ Device tensors, bfloat16 or float16; every call is queued on the current torch s
 work area from torch's allocator on that stream."""
 from __future__ import annotations
 
+import functools
+
 from . import _lib as X
 
 _TYPES = {}                                     # torch dtype -> the ABI's type, once torch is loaded
@@ -19,15 +21,37 @@ def _types():
     return _TYPES
 
 
-def _check(who: str, name: str, t, dtype, shape, device, dense: bool = False):
-    """t is a device tensor of this type and shape whose columns are adjacent (dense: contiguous)."""
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or t.device != device:
-        raise ValueError(f"{who}: {name} is {t.dtype} {list(t.shape)} on {t.device}, needs {dtype} {list(shape)} on {device}")
-    if dense:
-        if not t.is_contiguous():
-            raise ValueError(f"{who}: {name} must be contiguous")
-    elif t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1:
+@functools.lru_cache(maxsize=1024)
+def _attn_bytes(*sizes) -> int:
+    return X.load().otpu_attn_work_bytes(*sizes)
+
+
+@functools.lru_cache(maxsize=1024)
+def _evict_bytes(*sizes) -> int:
+    return X.load().otpu_kv_evict_work_bytes(*sizes)
+
+
+def _check(who: str, name: str, t, dtype, shape, dev: int):
+    """t is a tensor of this type and shape on device `dev`."""
+    if t.dtype != dtype or t.shape != shape or t.get_device() != dev:
+        raise ValueError(f"{who}: {name} is {t.dtype} {list(t.shape)} on {t.device}, needs {dtype} {list(shape)} on cuda:{dev}")
+
+
+def _dense(who: str, name: str, t, dtype, shape, dev: int) -> int:
+    """The address of a contiguous tensor."""
+    _check(who, name, t, dtype, shape, dev)
+    if not t.is_contiguous():
+        raise ValueError(f"{who}: {name} must be contiguous")
+    return t.data_ptr()
+
+
+def _rows(who: str, name: str, t, dtype, shape, dev: int) -> tuple:
+    """The strides of a tensor whose columns are adjacent."""
+    _check(who, name, t, dtype, shape, dev)
+    s = t.stride()
+    if s[-1] != 1 and t.numel() and shape[-1] > 1:
         raise ValueError(f"{who}: the columns of {name} must be adjacent")
+    return s
 
 
 def shared(q, prefix_k, prefix_v, k, v, lens, *, scale: float | None = None, weights=None, out=None):
@@ -41,46 +65,45 @@ def shared(q, prefix_k, prefix_v, k, v, lens, *, scale: float | None = None, wei
     own token's softmax weights, summed over the queries and the query heads of its head, are added to
     it.  out: a tensor to write to, which must overlap no input."""
     kinds = _types()
-    if q.dim() != 4 or not q.is_cuda or kinds.get(q.dtype, X.F32) == X.F32:
-        raise ValueError(f"shared: q is {q.dtype} {list(q.shape)} on {q.device}, needs [B, Lq, Hq, D] in bfloat16 or float16")
+    dt, dev = q.dtype, q.get_device()
+    if q.dim() != 4 or dev < 0 or kinds.get(dt, X.F32) == X.F32:
+        raise ValueError(f"shared: q is {dt} {list(q.shape)} on {q.device}, needs [B, Lq, Hq, D] in bfloat16 or float16")
     B, Lq, Hq, D = q.shape
-    dt, dev = q.dtype, q.device
     if (prefix_k is None) != (prefix_v is None) or (k is None) != (v is None) or (k is None) != (lens is None):
         raise ValueError("shared: prefix_k and prefix_v go together, so do k, v and lens")
     if prefix_k is None and k is None:
         raise ValueError("shared: neither a prefix nor a cache")
-    P = T = 0
-    Hkv = (k if prefix_k is None else prefix_k).shape[-2]
-    _check("shared", "q", q, dt, (B, Lq, Hq, D), dev)
-    pk = pv = kp = vp = lp = None
-    ps = ks = vs = (0, 0, 0)
-    pvs = (0, 0)
+    T = X.torch()
+    P = N = 0
+    pk = pv = kp = vp = lp = wp = None
+    ps = pvs = ks = vs = (0, 0, 0)
+    qs = _rows("shared", "q", q, dt, (B, Lq, Hq, D), dev)
+    if k is not None:
+        N, Hkv = k.shape[1], k.shape[-2]
+        ks = _rows("shared", "k", k, dt, (B, N, Hkv, D), dev)
+        vs = _rows("shared", "v", v, dt, (B, N, Hkv, D), dev)
+        lp = _dense("shared", "lens", lens, T.int32, (B,), dev)
+        kp, vp = k.data_ptr(), v.data_ptr()
+    else:
+        Hkv = prefix_k.shape[-2]
     if prefix_k is not None:
         P = prefix_k.shape[0]
-        _check("shared", "prefix_k", prefix_k, dt, (P, Hkv, D), dev)
-        _check("shared", "prefix_v", prefix_v, dt, (P, Hkv, D), dev)
-        pk, pv, ps, pvs = prefix_k.data_ptr(), prefix_v.data_ptr(), prefix_k.stride(), prefix_v.stride()
-    if k is not None:
-        T = k.shape[1]
-        _check("shared", "k", k, dt, (B, T, Hkv, D), dev)
-        _check("shared", "v", v, dt, (B, T, Hkv, D), dev)
-        _check("shared", "lens", lens, X.torch().int32, (B,), dev, True)
-        kp, vp, lp, ks, vs = k.data_ptr(), v.data_ptr(), lens.data_ptr(), k.stride(), v.stride()
+        ps = _rows("shared", "prefix_k", prefix_k, dt, (P, Hkv, D), dev)
+        pvs = _rows("shared", "prefix_v", prefix_v, dt, (P, Hkv, D), dev)
+        pk, pv = prefix_k.data_ptr(), prefix_v.data_ptr()
     if weights is not None:
-        _check("shared", "weights", weights, X.torch().float32, (B, Hkv, T), dev, True)
+        wp = _dense("shared", "weights", weights, T.float32, (B, Hkv, N), dev)
     if out is None:
-        out = X.torch().empty((B, Lq, Hq, D), dtype=dt, device=dev)
-    else:
-        _check("shared", "out", out, dt, (B, Lq, Hq, D), dev)
+        out = T.empty_like(q, memory_format=T.contiguous_format)
+    os = _rows("shared", "out", out, dt, (B, Lq, Hq, D), dev)
     if out.numel() == 0:
         return out
-    nbytes = X.load().otpu_attn_work_bytes(B, Lq, Hq, Hkv, D, P, T)
-    work = X.torch().empty((max(nbytes, 1),), dtype=X.torch().uint8, device=dev)
-    qs, os = q.stride(), out.stride()
+    nbytes = _attn_bytes(B, Lq, Hq, Hkv, D, P, N)
+    work = T.empty((max(nbytes, 1),), dtype=T.uint8, device=q.device)
     X.call("otpu_attn_shared", q.data_ptr(), qs[0], qs[1], qs[2], pk, ps[0], ps[1], pv, pvs[0], pvs[1], P, kp, ks[0],
-           ks[1], ks[2], vp, vs[0], vs[1], vs[2], lp, T, B, Lq, Hq, Hkv, D, kinds[dt],
-           D ** -0.5 if scale is None else scale, out.data_ptr(), os[0], os[1], os[2], X.ptr(weights), work.data_ptr(),
-           nbytes, X.stream())
+           ks[1], ks[2], vp, vs[0], vs[1], vs[2], lp, N, B, Lq, Hq, Hkv, D, kinds[dt],
+           D ** -0.5 if scale is None else scale, out.data_ptr(), os[0], os[1], os[2], wp, work.data_ptr(), nbytes,
+           X.stream())
     return out
 
 
@@ -94,26 +117,23 @@ def evict(k, v, weights, pos, lens, budget: int, recent: int = 0, *, out=None):
     it) and its token's position.  lens int32 [B].  Returns the new (weights, pos, lens); slots past the new
     length have weight 0 and position -1.  out: the three tensors to write them to; (weights, pos, lens)
     themselves may be given."""
-    kinds = _types()
-    if k.dim() != 4 or not k.is_cuda or k.dtype not in kinds:
-        raise ValueError(f"evict: k is {k.dtype} {list(k.shape)} on {k.device}, needs [B, T, H, D] in bfloat16, float16 or float32")
-    B, T, H, D = k.shape
-    t, dev, e = X.torch(), k.device, k.element_size()
-    _check("evict", "k", k, k.dtype, (B, T, H, D), dev)
-    _check("evict", "v", v, k.dtype, (B, T, H, D), dev)
+    dt, dev, T = k.dtype, k.get_device(), X.torch()
+    if k.dim() != 4 or dev < 0 or dt not in _types():
+        raise ValueError(f"evict: k is {dt} {list(k.shape)} on {k.device}, needs [B, T, H, D] in bfloat16, float16 or float32")
+    B, N, H, D = k.shape
+    e = k.element_size()
+    ks, vs = _rows("evict", "k", k, dt, (B, N, H, D), dev), _rows("evict", "v", v, dt, (B, N, H, D), dev)
+    slots = (B, H, N)
+    old = (_dense("evict", "weights", weights, T.float32, slots, dev), _dense("evict", "pos", pos, T.int32, slots, dev),
+           _dense("evict", "lens", lens, T.int32, (B,), dev))
     if out is None:
-        out = (t.empty_like(weights), t.empty_like(pos), t.empty_like(lens))
-    for name, x, dt, shape in (("weights", weights, t.float32, (B, H, T)), ("pos", pos, t.int32, (B, H, T)),
-                               ("lens", lens, t.int32, (B,))):
-        _check("evict", name, x, dt, shape, dev, True)
-    for name, x, dt, shape in zip(("out[0]", "out[1]", "out[2]"), out, (t.float32, t.int32, t.int32),
-                                  ((B, H, T), (B, H, T), (B,))):
-        _check("evict", name, x, dt, shape, dev, True)
-    nbytes = X.load().otpu_kv_evict_work_bytes(B, T, H, budget)
-    work = t.empty((max(nbytes, 1),), dtype=t.uint8, device=dev)
-    X.call("otpu_kv_evict", k.data_ptr(), *(e * s for s in k.stride()[:3]), v.data_ptr(), *(e * s for s in v.stride()[:3]),
-           e * D, weights.data_ptr(), pos.data_ptr(), lens.data_ptr(), B, T, H, budget, recent, out[0].data_ptr(),
-           out[1].data_ptr(), out[2].data_ptr(), work.data_ptr(), nbytes, X.stream())
+        out = (T.empty_like(weights), T.empty_like(pos), T.empty_like(lens))
+    new = (_dense("evict", "out[0]", out[0], T.float32, slots, dev), _dense("evict", "out[1]", out[1], T.int32, slots, dev),
+           _dense("evict", "out[2]", out[2], T.int32, (B,), dev))
+    nbytes = _evict_bytes(B, N, H, budget)
+    work = T.empty((max(nbytes, 1),), dtype=T.uint8, device=k.device)
+    X.call("otpu_kv_evict", k.data_ptr(), e * ks[0], e * ks[1], e * ks[2], v.data_ptr(), e * vs[0], e * vs[1], e * vs[2],
+           e * D, *old, B, N, H, budget, recent, *new, work.data_ptr(), nbytes, X.stream())
     return out
 
 

@@ -492,18 +492,18 @@ __global__ __launch_bounds__(NW * 64, DP <= 128 ? 2 : 1) void segment_kernel(Att
 }
 
 // The partials of a row joined: GP threads take every GP-th partial of four columns, their sums meet in
-// LDS.  Workgroups past the rows' add the own tokens' weights from the scores: 1024 tokens of a (sequence,
+// LDS.  The first nw workgroups add the own tokens' weights from the scores: 1024 tokens of a (sequence,
 // head) each, the rows' sums joined again.
 constexpr int WT = 1024;
 template <class E, int GP>
-__global__ __launch_bounds__(256) void combine_kernel(AttnArgs a, int nrows) {
+__global__ __launch_bounds__(256) void combine_kernel(AttnArgs a, int nw) {
     __shared__ float sm[256], sl[256];
     __shared__ v4f so[256];
     const int64_t rows = (int64_t)a.B * a.Lq * a.Hq;
     const int n = a.sp + a.ss, tid = threadIdx.x;
-    if ((int)blockIdx.x >= nrows) {
+    if ((int)blockIdx.x < nw) {
         const int R = a.Lq * a.G, nt = (a.T + WT - 1) / WT;
-        const int x = blockIdx.x - nrows, bh = x / nt, t0 = x % nt * WT;
+        const int x = blockIdx.x, bh = x / nt, t0 = x % nt * WT;
         const int b = bh / a.Hkv, h = bh - b * a.Hkv;
         const int len = min(max(a.lens[b], 0), a.T);
         if (t0 >= len) return;
@@ -531,12 +531,18 @@ __global__ __launch_bounds__(256) void combine_kernel(AttnArgs a, int nrows) {
         if (t >= len) return;
         const float* const sc = a.sc + (int64_t)bh * R * a.tp + t;
         v4f w = {0.f, 0.f, 0.f, 0.f};
-        for (int r = 0; r < R; ++r) {
-            const int see = len - a.Lq + r / a.G;           // the row's own token
-            const v4f s = *reinterpret_cast<const v4f*>(sc + (int64_t)r * a.tp);
+        for (int r0 = 0; r0 < R; r0 += 8) {
+            v4f s[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (t + j <= see) w[j] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], a.scale2, -sm[r]));
+            for (int u = 0; u < 8; ++u) s[u] = *reinterpret_cast<const v4f*>(sc + (int64_t)min(r0 + u, R - 1) * a.tp);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int see = r0 + u < R ? len - a.Lq + (r0 + u) / a.G : -1;   // the row's own token
+                const float lse = sm[min(r0 + u, R - 1)];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (t + j <= see) w[j] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][j], a.scale2, -lse));
+            }
         }
         float* const out = a.weights + (int64_t)bh * a.T + t;
 #pragma unroll
@@ -546,7 +552,7 @@ __global__ __launch_bounds__(256) void combine_kernel(AttnArgs a, int nrows) {
     }
     const int per = a.D / 4, rpb = 256 / (per * GP);       // rows a workgroup
     const int rl = tid / (per * GP), y = tid - rl * per * GP, g = y / per, d = (y - g * per) * 4;
-    const int64_t row = (int64_t)blockIdx.x * rpb + rl;
+    const int64_t row = (int64_t)(blockIdx.x - nw) * rpb + rl;
     const bool ok = rl < rpb && row < rows;
     float m = -__builtin_inff(), l = 0.f;
     v4f o = {0.f, 0.f, 0.f, 0.f};
@@ -715,7 +721,7 @@ static void launch_combine(const AttnArgs& a, const Plan& p, hipStream_t s) {
     const int rpb = 256 / (a.D / 4 * GP);
     const int nrows = (int)((p.rows + rpb - 1) / rpb);
     const int nw = a.sc ? a.B * a.Hkv * ((a.T + WT - 1) / WT) : 0;
-    combine_kernel<E, GP><<<nrows + nw, 256, 0, s>>>(a, nrows);
+    combine_kernel<E, GP><<<nrows + nw, 256, 0, s>>>(a, nw);
 }
 
 template <class E, int DP, bool FULL>

@@ -218,27 +218,32 @@ def norm_quantize(x, gamma, residual=None, *, eps: float = 1e-6, row_mode: bool 
     if X.is_numpy(x):
         x = X.dev(x, np.float32)
         residual = None if residual is None else X.dev(residual, np.float32)
-    dt = x.dtype
-    if dt not in NORM_TYPES or x.dim() != 2 or not x.is_cuda:
+    dt, dev = x.dtype, x.get_device()
+    if dt not in NORM_TYPES or x.dim() != 2 or dev < 0:
         raise ValueError(f"norm_quantize: x is {dt} {list(x.shape)} on {x.device}, needs [M, K] in float32, bfloat16 or float16")
-    M, K = x.shape
-    g = gamma if isinstance(gamma, T.Tensor) and gamma.dtype == T.float32 and gamma.is_contiguous() else X.dev(gamma, np.float32)
-    if g.shape != (K,):
-        raise ValueError(f"norm_quantize: gamma {list(g.shape)} over {K} columns")
-    if h is None and residual is not None:
-        h = T.empty((M, K), dtype=dt, device=x.device)
-    for name, t in (("x", x), ("residual", residual), ("h", h)):
-        if t is not None and (t.dtype != dt or t.shape != x.shape or t.device != x.device or (K > 1 and t.stride(1) != 1)):
+    M, K = shape = x.shape
+
+    def row(name, t):
+        s = t.stride()
+        if t is not x and (t.dtype != dt or t.shape != shape or t.get_device() != dev) or (s[1] != 1 and K > 1):
             raise ValueError(f"norm_quantize: {name} is {t.dtype} {list(t.shape)} on {t.device}, needs {dt} {[M, K]} on "
-                             f"{x.device}, columns adjacent")
-    if r is not None and (r.dtype != T.float32 or r.shape != (M,) or not r.is_contiguous() or r.device != x.device):
+                             f"cuda:{dev}, columns adjacent")
+        return t.data_ptr(), s[0]
+
+    if not (isinstance(gamma, T.Tensor) and gamma.dtype == T.float32 and gamma.is_contiguous() and gamma.get_device() == dev):
+        gamma = X.dev(gamma, np.float32)
+    if gamma.shape != (K,):
+        raise ValueError(f"norm_quantize: gamma {list(gamma.shape)} over {K} columns")
+    if h is None and residual is not None:
+        h = T.empty_like(x, memory_format=T.contiguous_format)
+    xp, rp, hp = row("x", x), (None, 0) if residual is None else row("residual", residual), (None, 0) if h is None else row("h", h)
+    if r is not None and (r.dtype != T.float32 or r.shape != (M,) or not r.is_contiguous() or r.get_device() != dev):
         raise ValueError("norm_quantize: r is a contiguous float32 tensor [M]")
-    q = T.empty((M, K), dtype=T.int8, device=x.device)
-    d = T.empty((M, K // 32), dtype=T.uint8, device=x.device)
+    q = T.empty_like(x, dtype=T.int8, memory_format=T.contiguous_format)
     S = T.empty((1, M), dtype=T.float32, device=x.device)
-    X.call("otpu_norm_qact", x.data_ptr(), x.stride(0), X.ptr(residual), 0 if residual is None else residual.stride(0),
-           NORM_TYPES[dt], M, K, g.data_ptr(), eps, X.Q_ROW if row_mode else 0, X.ptr(h), 0 if h is None else h.stride(0),
-           X.ptr(r), q.data_ptr(), K, S.data_ptr(), d.data_ptr(), K // 32, X.stream())
+    d = T.empty((M, K // 32), dtype=T.uint8, device=x.device)
+    X.call("otpu_norm_qact", *xp, *rp, NORM_TYPES[dt], M, K, gamma.data_ptr(), eps, X.Q_ROW if row_mode else 0, *hp,
+           None if r is None else r.data_ptr(), q.data_ptr(), K, S.data_ptr(), d.data_ptr(), K // 32, X.stream())
     return _operand(q, S, d, [K], bool(row_mode)), x if h is None else h
 
 
