@@ -5,8 +5,9 @@
 // holes are filled, sources and destinations are disjoint and every move is independent.
 //
 //   evict_select_kernel   a workgroup a (sequence, head): the threshold by radix selection (11, 11 and 10
-//                         bits), the holes and their sources, the slots' weights and positions
-//   evict_move_kernel     the rows of k and v, 16 bytes a lane
+//                         bits), the holes and their sources, the slots' weights and positions; up to 64
+//                         rows of k and v
+//   evict_move_kernel     more rows of k and v
 #include "otpu_common.h"
 
 namespace otpu {
@@ -15,6 +16,7 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
 constexpr int EW = 1024;                     // threads of a selecting workgroup
 constexpr int BINS = 2048;
+constexpr int HERE = 64;                     // moves that the selecting workgroup makes itself
 
 struct EvictArgs {
     char* k; int64_t kb, kt, kh;             // byte strides of sequence, slot, head
@@ -28,6 +30,7 @@ struct EvictArgs {
     int* count;                              // [B H] moves
     int2* moves;                             // [B H][most] (to, from)
     int most;
+    bool here;                               // few moves: the selecting workgroup makes them
 };
 
 // weights in the order of the selection: NaN above infinity, -0 with +0
@@ -37,7 +40,8 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return (u >> 31) ? ~u : (u | 0x80000000u);
 }
 
-// exclusive sum of v over the workgroup's threads, in thread order; total: the whole sum
+// exclusive sum of v over the workgroup's threads, in thread order; total: the whole sum.  tmp: EW / 64
+// words that the next call does not use
 __device__ __forceinline__ int block_scan(int v, int* tmp, int& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int x = v;
@@ -49,28 +53,64 @@ __device__ __forceinline__ int block_scan(int v, int* tmp, int& total) {
     if (lane == 63) tmp[wave] = x;
     __syncthreads();
     int before = 0, all = 0;
+#pragma unroll
     for (int i = 0; i < EW / 64; ++i) {
         const int t = tmp[i];
         before += i < wave ? t : 0;
         all += t;
     }
-    __syncthreads();
     total = all;
     return before + x - v;
 }
 
-__global__ __launch_bounds__(EW) void evict_select_kernel(EvictArgs a) {
-    __shared__ int hist[BINS];
-    __shared__ int tmp[EW / 64];
+// rows of k and v from slot m.y to slot m.x, `c` pieces of 16 bytes each: threads in groups of c (or all of
+// them for one row), several rows' loads out at once
+template <int THREADS, int U>
+__device__ __forceinline__ void move_rows(const EvictArgs& a, char* k, char* v, const int2* mv, int n, int first, int step) {
+    const int c = a.row / 16, per = c < THREADS ? THREADS / c : 1;      // rows at once
+    const int g = threadIdx.x / (c < THREADS ? c : THREADS), x0 = threadIdx.x - g * c;
+    if (g >= per) return;
+    for (int j0 = first * per + g; j0 < n; j0 += U * step * per) {
+        int2 m[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) m[u] = mv[min(j0 + u * step * per, n - 1)];
+        for (int x = x0; x < c; x += THREADS) {
+            v4u kk[U], vv[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                kk[u] = *reinterpret_cast<const v4u*>(k + m[u].y * a.kt + 16 * x);
+                vv[u] = *reinterpret_cast<const v4u*>(v + m[u].y * a.vt + 16 * x);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (j0 + u * step * per < n) {
+                    *reinterpret_cast<v4u*>(k + m[u].x * a.kt + 16 * x) = kk[u];
+                    *reinterpret_cast<v4u*>(v + m[u].x * a.vt + 16 * x) = vv[u];
+                }
+        }
+    }
+}
+
+// KPT keys a thread in registers, slots in turn over the threads; a cache of more than KPT * 1024 slots in
+// such chunks, its keys read again for each pass over them.
+template <int KPT>
+__global__ __launch_bounds__(EW, KPT <= 8 ? 8 : 4) void evict_select_kernel(EvictArgs a) {
+    constexpr int WV = EW / 64;
+    // four counts a digit, by lane: weights lie in few digits, and one address takes one lane at a time
+    __shared__ __attribute__((aligned(16))) int hist[4 * BINS];
+    __shared__ int2 few[HERE];               // few moves
+    __shared__ int tmp[2][WV];
+    __shared__ int cnt[KPT * WV];
     __shared__ uint32_t digit;
-    __shared__ int above;
-    const int tid = threadIdx.x;
+    __shared__ int above, equal;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int bh = blockIdx.x, b = bh / a.H;
     const int n = min(max(a.lens[b], 0), a.T), left = min(n, a.budget);
     const float* const w = a.w + (int64_t)bh * a.T;
     const int32_t* const pos = a.pos + (int64_t)bh * a.T;
     float* const wn = a.wn + (int64_t)bh * a.T;
     int32_t* const pn = a.pn + (int64_t)bh * a.T;
+    if (tid == 0 && bh % a.H == 0 && a.ln != a.lens) a.ln[b] = left;
 
     if (n <= a.budget || a.budget == 0) {    // every slot stays, or none
         for (int t = tid; t < a.T; t += EW) {
@@ -80,99 +120,179 @@ __global__ __launch_bounds__(EW) void evict_select_kernel(EvictArgs a) {
         if (tid == 0) a.count[bh] = 0;
         return;
     }
-    // the newest position
-    int64_t newest = INT32_MIN;
-    for (int t = tid; t < n; t += EW) newest = max(newest, (int64_t)pos[t]);
+    for (int i = tid; i < BINS; i += EW) reinterpret_cast<int4*>(hist)[i] = make_int4(0, 0, 0, 0);
+    const int chunks = (n + EW * KPT - 1) / (EW * KPT);
+    uint32_t key[KPT];
+    int32_t newest = INT32_MIN;              // the newest position
+    // positions and weights come in one trip where registers hold both, else the positions twice
+    constexpr bool HOLD = KPT <= 16;
+    int32_t ps[HOLD ? KPT : 1];
+    auto slot = [&](int c, int i) __attribute__((always_inline)) { return min((c * KPT + i) * EW + tid, n - 1); };
+    auto load = [&](int c) __attribute__((always_inline)) {
+        if constexpr (HOLD) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) newest = max(newest, (int64_t)__shfl_xor((int)newest, o, 64));
-    if ((tid & 63) == 0) tmp[tid >> 6] = (int)newest;
-    __syncthreads();
-    for (int i = 0; i < EW / 64; ++i) newest = max(newest, (int64_t)tmp[i]);
-    __syncthreads();
-    const int64_t old = newest - a.recent;   // positions past it stay
-    auto key = [&](int t) __attribute__((always_inline)) {
-        return (int64_t)pos[t] > old ? 0xFFFFFFFFu : weight_key(w[t]);
+            for (int i = 0; i < KPT; ++i) ps[i] = pos[slot(c, i)];
+#pragma unroll
+            for (int i = 0; i < KPT; ++i) key[i] = fbits(w[slot(c, i)]);
+        }
     };
+    for (int c = 0; c < chunks; ++c) {
+        load(c);
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) newest = max(newest, HOLD ? ps[HOLD ? i : 0] : pos[slot(c, i)]);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) newest = max(newest, __shfl_xor(newest, o, 64));
+    if (lane == 0) tmp[0][wave] = newest;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WV; ++i) newest = max(newest, tmp[0][i]);
+    const int64_t old = (int64_t)newest - a.recent;          // positions past it stay
+    // key 0: no slot (a weight's key is at least that of -inf)
+    auto keys = [&](int c) __attribute__((always_inline)) {
+        if (chunks > 1) load(c);
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) {
+            const int32_t p = HOLD ? ps[HOLD ? i : 0] : pos[slot(c, i)];
+            const uint32_t k = (int64_t)p > old ? 0xFFFFFFFFu : weight_key(HOLD ? bitsf(key[i]) : w[slot(c, i)]);
+            key[i] = (c * KPT + i) * EW + tid < n ? k : 0u;
+        }
+    };
+    if (chunks == 1) keys(0);
 
     // the key of the left-th slot, and how many of the slots with that key stay
     uint32_t prefix = 0, mask = 0;
-    int need = left;
+    int need = left, same = 0;
+#pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
-        const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
-        for (int i = tid; i < BINS; i += EW) hist[i] = 0;
-        __syncthreads();
-        for (int t = tid; t < n; t += EW) {
-            const uint32_t x = key(t);
-            if ((x & mask) == prefix) atomicAdd(&hist[(x >> shift) & ((1u << bits) - 1)], 1);
+        const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
+        const uint32_t dm = pass == 2 ? 0x3FFu : 0x7FFu;
+#pragma unroll 1
+        for (int c = 0; c < chunks; ++c) {
+            if (chunks > 1) keys(c);
+#pragma unroll
+            for (int i = 0; i < KPT; ++i)      // (key 0 is below every slot's: never chosen)
+                if ((key[i] & mask) == prefix) atomicAdd(&hist[4 * ((key[i] >> shift) & dm) + (lane & 3)], 1);
         }
         __syncthreads();
         // from the largest digit down: thread i sums digits 2047 - 2i and 2046 - 2i
-        const int c0 = hist[BINS - 1 - 2 * tid], c1 = hist[BINS - 2 - 2 * tid];
+        int4* const h4 = reinterpret_cast<int4*>(hist) + (BINS - 2 - 2 * tid);
+        const int4 lo = h4[0], hi = h4[1];
+        h4[0] = h4[1] = make_int4(0, 0, 0, 0);
+        const int c0 = hi.x + hi.y + hi.z + hi.w, c1 = lo.x + lo.y + lo.z + lo.w;
         int total;
-        const int before = block_scan(c0 + c1, tmp, total);
+        const int before = block_scan(c0 + c1, tmp[1 - (pass & 1)], total);
         if (before < need && before + c0 + c1 >= need) {
             const bool first = before + c0 >= need;
             digit = (uint32_t)(first ? BINS - 1 - 2 * tid : BINS - 2 - 2 * tid);
             above = first ? before : before + c0;
+            equal = first ? c0 : c1;
         }
         __syncthreads();
         prefix |= digit << shift;
-        mask |= ((1u << bits) - 1) << shift;
+        mask |= dm << shift;
         need -= above;
-        __syncthreads();
+        same = equal;
+        if (same == need) break;              // (uniform) all of this digit's slots stay: no ties
     }
 
-    // in slot order: which of the equal keys stay, the holes and the sources
-    int2* const mv = a.moves + (int64_t)bh * a.most;
+    // in slot order: which of the equal keys stay, the holes and the sources.  cnt: a wave's count at each of
+    // its KPT places, summed in slot order
+    int2* const mv = a.here ? few : a.moves + (int64_t)bh * a.most;
     int ties = 0, holes = 0, extras = 0;
-    for (int t0 = 0; t0 < n; t0 += EW) {
-        const int t = t0 + tid;
-        const uint32_t x = t < n ? key(t) : 0u;
-        const bool tie = t < n && x == prefix;
+    const uint64_t below = (1ull << lane) - 1;
+    auto ordered = [&]() __attribute__((always_inline)) {    // cnt: exclusive sums; returns the whole sum
+        __syncthreads();
+        const int mine = tid < KPT * WV ? cnt[tid] : 0;
         int total;
-        const int before = block_scan(tie ? 1 : 0, tmp, total);
-        const bool stays = t < n && (x > prefix || (tie && ties + before < need));
-        ties += total;
-        const bool hole = t < left && !stays, extra = t >= left && stays;
-        int tot;
-        const int at = block_scan((hole ? 1 : 0) | (extra ? 1 << 16 : 0), tmp, tot);
-        if (hole) mv[holes + (at & 0xFFFF)].x = t;
-        if (extra) mv[extras + (at >> 16)].y = t;
-        holes += tot & 0xFFFF;
-        extras += tot >> 16;
-        if (t < left && stays && wn != w) { wn[t] = w[t]; pn[t] = pos[t]; }
+        const int x = block_scan(mine, tmp[0], total);
+        if (tid < KPT * WV) cnt[tid] = x;
+        __syncthreads();
+        return total;
+    };
+#pragma unroll 1
+    for (int c = 0; c < chunks; ++c) {
+        if (chunks > 1) keys(c);
+        uint32_t stay = 0;                                   // bit i: the slot at place i stays
+        if (same == need) {
+#pragma unroll
+            for (int i = 0; i < KPT; ++i) stay |= (uint32_t)(key[i] >= prefix) << i;
+        } else {
+#pragma unroll
+            for (int i = 0; i < KPT; ++i) {
+                const int v = __builtin_popcountll(__ballot(key[i] == prefix));
+                if (lane == 0) cnt[i * WV + wave] = v;
+            }
+            const int total = ordered();
+#pragma unroll
+            for (int i = 0; i < KPT; ++i) {
+                const bool tie = key[i] == prefix;
+                const int rank = ties + cnt[i * WV + wave] + __builtin_popcountll(__ballot(tie) & below);
+                stay |= (uint32_t)(key[i] > prefix || (tie && rank < need)) << i;
+            }
+            ties += total;
+            __syncthreads();
+        }
+        // a slot below `left` that goes, or one at or past it that stays
+        int t0 = c * KPT * EW + tid;
+        // (both as values in a register: a mask a slot, kept over the barriers, takes more scalar ones than
+        // there are)
+        asm volatile("" : "+v"(stay));
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) {
+            const bool s = (stay >> i) & 1, low = t0 + i * EW < left;
+            const int v = __builtin_popcountll(__ballot(low && !s)) | __builtin_popcountll(__ballot(!low && s)) << 16;
+            if (lane == 0) cnt[i * WV + wave] = v;
+        }
+        const int total = ordered();
+        asm volatile("" : "+v"(stay), "+v"(t0));
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) {
+            const int t = t0 + i * EW, at = cnt[i * WV + wave];
+            const bool s = (stay >> i) & 1, low = t < left;
+            const uint64_t holes_of = __ballot(low && !s), extras_of = __ballot(!low && s);
+            if (low && !s) mv[holes + (at & 0xFFFF) + __builtin_popcountll(holes_of & below)].x = t;
+            if (!low && s) mv[extras + (at >> 16) + __builtin_popcountll(extras_of & below)].y = t;
+            if (low && s && wn != w) { wn[t] = w[t]; pn[t] = pos[t]; }
+        }
+        holes += total & 0xFFFF;
+        extras += total >> 16;
     }
-    __threadfence_block();
     __syncthreads();
     for (int j = tid; j < holes; j += EW) {
         const int2 m = mv[j];
         wn[m.x] = w[m.y];
         pn[m.x] = pos[m.y];
     }
+    if (a.here) move_rows<EW, 1>(a, a.k + b * a.kb + (bh - b * a.H) * a.kh, a.v + b * a.vb + (bh - b * a.H) * a.vh, mv, holes, 0, 1);
     __syncthreads();
     for (int t = left + tid; t < a.T; t += EW) { wn[t] = 0.f; pn[t] = -1; }
     if (tid == 0) a.count[bh] = holes;
 }
 
-__global__ __launch_bounds__(256) void evict_lens_kernel(const int32_t* lens, int32_t* ln, int B, int T, int budget) {
-    const int b = blockIdx.x * 256 + threadIdx.x;
-    if (b < B) ln[b] = min(min(max(lens[b], 0), T), budget);
+// the lengths in place, when no workgroup reads them any more
+__device__ __forceinline__ void store_lens(const EvictArgs& a) {
+    if (a.ln != a.lens) return;
+    for (int b = threadIdx.x; b < a.B; b += 256) a.ln[b] = min(min(max(a.lens[b], 0), a.T), a.budget);
 }
+__global__ __launch_bounds__(256) void evict_lens_kernel(EvictArgs a) { store_lens(a); }
 
 __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
     const int bh = blockIdx.x, b = bh / a.H, h = bh - b * a.H;
-    const int n = a.count[bh], c = a.row / 16;
-    const int2* const mv = a.moves + (int64_t)bh * a.most;
-    char* const k = a.k + b * a.kb + h * a.kh;
-    char* const v = a.v + b * a.vb + h * a.vh;
-    for (int64_t i = (int64_t)blockIdx.y * 256 + threadIdx.x; i < (int64_t)n * c; i += (int64_t)gridDim.y * 256) {
-        const int j = (int)(i / c), x = (int)(i - (int64_t)j * c) * 16;
-        const int2 m = mv[j];
-        const v4u kk = *reinterpret_cast<const v4u*>(k + m.y * a.kt + x);
-        const v4u vv = *reinterpret_cast<const v4u*>(v + m.y * a.vt + x);
-        *reinterpret_cast<v4u*>(k + m.x * a.kt + x) = kk;
-        *reinterpret_cast<v4u*>(v + m.x * a.vt + x) = vv;
-    }
+    if (bh == 0 && blockIdx.y == 0) store_lens(a);
+    move_rows<256, 4>(a, a.k + b * a.kb + h * a.kh, a.v + b * a.vb + h * a.vh, a.moves + (int64_t)bh * a.most, a.count[bh],
+                   blockIdx.y, gridDim.y);
+}
+
+static void launch_select(const EvictArgs& a, hipStream_t s) {
+    const unsigned grid = (unsigned)(a.B * a.H);
+    const int per = (a.T + EW - 1) / EW;
+    if (per <= 1) evict_select_kernel<1><<<grid, EW, 0, s>>>(a);
+    else if (per <= 2) evict_select_kernel<2><<<grid, EW, 0, s>>>(a);
+    else if (per <= 4) evict_select_kernel<4><<<grid, EW, 0, s>>>(a);
+    else if (per <= 8) evict_select_kernel<8><<<grid, EW, 0, s>>>(a);
+    else if (per <= 16) evict_select_kernel<16><<<grid, EW, 0, s>>>(a);
+    else evict_select_kernel<32><<<grid, EW, 0, s>>>(a);
 }
 
 }  // namespace otpu
@@ -222,12 +342,15 @@ extern "C" int otpu_kv_evict(void* k, int64_t kb, int64_t kt, int64_t kh, void* 
     a.count = (int*)work;
     a.moves = (int2*)((char*)work + ((4 * (int64_t)B * H + 255) & ~(int64_t)255));
     const hipStream_t s = (hipStream_t)stream;
-    if (T) evict_select_kernel<<<(unsigned)(B * H), EW, 0, s>>>(a);
-    if (a.most) {
-        const int64_t pieces = ((int64_t)a.most * (row_bytes / 16) + 255) / 256;
+    a.here = a.most <= HERE;
+    if (T) launch_select(a, s);
+    if (T && !a.here) {
+        const int c = row_bytes / 16, per = c < 256 ? 256 / c : 1;
+        const int64_t pieces = (a.most + per - 1) / per;
         const int64_t want = (8 * (int64_t)otpu_cu_count() + B * H - 1) / ((int64_t)B * H);
         evict_move_kernel<<<dim3((unsigned)(B * H), (unsigned)(pieces < want ? pieces : want)), 256, 0, s>>>(a);
+    } else if (lens_out == lens || !T) {
+        evict_lens_kernel<<<1, 256, 0, s>>>(a);
     }
-    evict_lens_kernel<<<(B + 255) / 256, 256, 0, s>>>(lens, lens_out, B, T, budget);
     return otpu_launch_check("kv_evict");
 }
