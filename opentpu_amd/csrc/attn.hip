@@ -52,7 +52,7 @@ struct AttnArgs {
     float scale2;                            // scale * log2(e)
     int sp, ss, per_p;                       // splits of the prefix, of the own keys; keys of a prefix split
     uint32_t np, no;                         // workgroups of the prefix, of the own keys
-    bool keys_p, keys_o;                     // their shape
+    int rows_p, rows_o;                      // rows of their tiles: 32 or 128
     float* po;                               // partial o [sp + ss][rows][D]
     float* pm;                               // m [sp + ss][rows]
     float* pl;                               // l [sp + ss][rows]
@@ -101,10 +101,11 @@ template <int DP_> struct Shape {
     static constexpr int LDS = ROWS_LDS > KEYS_LDS ? ROWS_LDS : KEYS_LDS;
 };
 
-// chunk c of key row r lies in slot c ^ f(r): the 8 (16) rows that lanes read together at one c on
-// distinct banks; of value row r: the 4 rows that a transposing read takes, two chunks each
-template <int CR> __device__ __forceinline__ int kswz(int r) { return r & (CR < 16 ? CR - 1 : 15); }
-template <int CR> __device__ __forceinline__ int vswz(int r) { return (2 * r) & (CR < 16 ? CR - 1 : 15); }
+// Chunk c of row r lies in slot c ^ f(r).  LDS serves 256 bytes a cycle from 64 banks.  Keys: the 16 rows
+// that 16 lanes read at one c in 16 different slots (rows of 128 bytes: slots of both row parities).
+// Values: the 4 rows by 4 chunks that 32 lanes of a transposing read take, likewise.
+template <int CR> __device__ __forceinline__ int kswz(int r) { return CR < 16 ? (r >> 1) & 7 : r & 15; }
+template <int CR> __device__ __forceinline__ int vswz(int r) { return CR < 16 ? 4 * ((r >> 1) & 1) : 4 * (r & 3); }
 
 // Direct loads of `rows` rows of a segment from row r0 on into LDS at `to`, dealt to nw waves of which
 // this is number w; rows past `last` read it instead.
@@ -157,39 +158,33 @@ __device__ __forceinline__ void finite_values(char* vs, int pieces, int* flag) {
     }
 }
 
-// One step: 32 TT keys at ks and their values at vs (LDS) from the segment's key `at` on.  lim: the
-// segment's keys that this lane's row sees; first: the least of the wave's, least: of the workgroup's.
-// keys_read() runs once the keys are read, values_come() before the values are.  sc: the scores' row (or
-// NULL), for the weights.
-template <class E, int DP, int TT, bool OWN, class FK, class FV>
-__device__ __forceinline__ void step(Acc<DP>& a, const char* ks, const char* vs, int at, int lim, int first,
-                                     int least, int* flag, const v8s (&qf)[DP / 16], float c2, float* sc, FK keys_read,
-                                     FV values_come) {
-    constexpr int CR = DP / 8, KS = DP / 16, DT = DP / 32;
+// S^T = K Q^T of 32 TT keys at ks (LDS): a lane has its row's scores of keys 8 r + 4 hh + 0..3 of each 32
+template <class E, int DP, int TT>
+__device__ __forceinline__ void scores(v16f (&s)[TT], const char* ks, const v8s (&qf)[DP / 16]) {
+    constexpr int CR = DP / 8;
     const int lane = threadIdx.x & 63, r32 = lane & 31, hh = lane >> 5;
-    v16f s[TT];
 #pragma unroll
-    for (int t = 0; t < TT; ++t) {
+    for (int t = 0; t < TT; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
-        const int kr = t * 32 + r32;
 #pragma unroll
-        for (int x = 0; x < KS; ++x) {
+    for (int x = 0; x < DP / 16; ++x) {
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+            const int kr = t * 32 + r32;
             const v8s kf = *reinterpret_cast<const v8s*>(ks + kr * (DP * 2) + (((2 * x + hh) ^ kswz<CR>(kr)) << 4));
             s[t] = E::mma(kf, qf[x], s[t]);
         }
     }
-    keys_read();
-    if (OWN && sc) {
-#pragma unroll
-        for (int t = 0; t < TT; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                *reinterpret_cast<v4f*>(sc + at + t * 32 + 8 * r + 4 * hh) =
-                    v4f{s[t][4 * r], s[t][4 * r + 1], s[t][4 * r + 2], s[t][4 * r + 3]};
-    }
-    const bool masked = at + 32 * TT > first;              // (uniform) keys that a row does not see
-    if (masked) {
+}
+
+// The running softmax over the scores of the segment's keys from `at` on: m, l and o brought up to date,
+// the weights rounded to 16 bits for the product.  lim: the segment's keys that this lane's row sees;
+// first: the least of the wave's.
+template <class E, int DP, int TT>
+__device__ __forceinline__ void softmax(Acc<DP>& a, v16f (&s)[TT], v8s (&p)[2 * TT], int at, int lim, int first, float c2) {
+    const int hh = (threadIdx.x >> 5) & 1;
+    if (at + 32 * TT > first) {                            // (uniform) keys that a row does not see
 #pragma unroll
         for (int t = 0; t < TT; ++t)
 #pragma unroll
@@ -210,7 +205,7 @@ __device__ __forceinline__ void step(Acc<DP>& a, const char* ks, const char* vs,
         a.m = mn;
         a.l *= al;
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
+        for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
             for (int r = 0; r < 16; ++r) a.o[t][r] *= al;
     }
@@ -218,35 +213,38 @@ __device__ __forceinline__ void step(Acc<DP>& a, const char* ks, const char* vs,
 #pragma unroll
     for (int t = 0; t < TT; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], c2, -mu));
-            a.l += s[t][r];
-        }
-    values_come();
-    // o^T += V^T P^T: registers 8j .. 8j+7 of a score tile are this lane's keys 16j + 4 hh + 0..3
-    // and 16j + 8 + 4 hh + 0..3, the order in which the values' transposing reads give them
-    auto values = [&](int t, int j, int d) INL {
-        typedef __attribute__((address_space(3))) v4s lv4s;
-        const int kr = t * 32 + 16 * j + 4 * hh + (lane & 15) / 4;
-        const int c = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-        const char* const p0 = vs + kr * (DP * 2) + ((c ^ vswz<CR>(kr)) << 4) + 8 * (lane & 1);
-        const char* const p1 = vs + (kr + 8) * (DP * 2) + ((c ^ vswz<CR>(kr + 8)) << 4) + 8 * (lane & 1);
-        const v4s a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s*)p0);
-        const v4s a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s*)p1);
-        return __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
-    };
-    if (OWN && at + 32 * TT > least) finite_values<E>(const_cast<char*>(vs), 32 * TT * CR, flag);
-#pragma unroll
-    for (int t = 0; t < TT; ++t)
-#pragma unroll
         for (int j = 0; j < 2; ++j) {
-            typename E::v8 p;
+            typename E::v8 w;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] = (typename E::e)s[t][8 * j + e];
-            const v8s pb = __builtin_bit_cast(v8s, p);
-#pragma unroll
-            for (int d = 0; d < DT; ++d) a.o[d] = E::mma(values(t, j, d), pb, a.o[d]);
+            for (int e = 0; e < 8; ++e) {
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][8 * j + e], c2, -mu));
+                a.l += x;
+                w[e] = (typename E::e)x;
+            }
+            p[2 * t + j] = __builtin_bit_cast(v8s, w);
         }
+}
+
+// o^T += V^T P^T of the values at vs (LDS): p's eight weights are this lane's keys 16j + 4 hh + 0..3 and
+// 16j + 8 + 4 hh + 0..3, the order in which the values' transposing reads give them
+template <class E, int DP, int TT>
+__device__ __forceinline__ void product(Acc<DP>& a, const char* vs, const v8s (&p)[2 * TT]) {
+    constexpr int CR = DP / 8;
+    typedef __attribute__((address_space(3))) v4s lv4s;
+    const int lane = threadIdx.x & 63, hh = lane >> 5;
+#pragma unroll
+    for (int j = 0; j < 2 * TT; ++j) {
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {
+            const int kr = 16 * j + 4 * hh + (lane & 15) / 4;
+            const int c = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+            const char* const p0 = vs + kr * (DP * 2) + ((c ^ vswz<CR>(kr)) << 4) + 8 * (lane & 1);
+            const char* const p1 = vs + (kr + 8) * (DP * 2) + ((c ^ vswz<CR>(kr + 8)) << 4) + 8 * (lane & 1);
+            const v4s a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s*)p0);
+            const v4s a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s*)p1);
+            a.o[d] = E::mma(__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7), p[j], a.o[d]);
+        }
+    }
 }
 
 // One workgroup's part: keys [key0, key1) of a segment for a tile of rows.
@@ -347,10 +345,15 @@ __device__ __forceinline__ void rows_part(const AttnArgs& a, char* lds, const Pa
         wait_dma<0>();
         bar();
         if (i + 1 < steps) issue(i + 1);
-        const char* const ks = lds + (i & 1) * 2 * S::RB;
+        char* const ks = lds + (i & 1) * 2 * S::RB;
         const int at = p.key0 + i * KT;
         if (OWN && at >= none) continue;                   // (uniform over the wave) no row of it sees these keys
-        step<E, DP, KT / 32, OWN>(c, ks, ks + S::RB, at, p.lim, first, p.least, flag, qf, a.scale2, nullptr, [] {}, [] {});
+        v16f s[KT / 32];
+        v8s w[KT / 16];
+        scores<E, DP>(s, ks, qf);
+        softmax<E>(c, s, w, at, p.lim, first, a.scale2);
+        if (OWN && at + KT > p.least) finite_values<E>(ks + S::RB, KT * CR, flag);
+        product<E, DP, KT / 32>(c, ks + S::RB, w);
     }
     store_part<DP, FULL>(a, c, swap32_sum(c.l), p);
     if constexpr (OWN) {
@@ -382,15 +385,23 @@ __device__ __forceinline__ void keys_part(const AttnArgs& a, char* lds, const Pa
     for (int j = wave; j < tiles; j += NW) {
         const bool more = j + NW < tiles;
         wait_dma<LOADS>();                                 // the keys are there; the values' loads are younger
-        step<E, DP, 1, OWN>(c, ks, vs, p.key0 + 32 * j, p.lim, first, p.least, flag, qf, a.scale2, p.sc,
-            [&]() INL {
-                asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-                if (more) keys(j + NW);
-            },
-            [&]() INL {
-                if (more) wait_dma<LOADS>();               // (the next keys' loads are younger)
-                else wait_dma<0>();
-            });
+        const int at = p.key0 + 32 * j;
+        v16f s[1];
+        v8s w[2];
+        scores<E, DP>(s, ks, qf);
+        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+        if (more) keys(j + NW);
+        if (OWN && p.sc) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                *reinterpret_cast<v4f*>(p.sc + at + 8 * r + 4 * (lane >> 5)) =
+                    v4f{s[0][4 * r], s[0][4 * r + 1], s[0][4 * r + 2], s[0][4 * r + 3]};
+        }
+        softmax<E>(c, s, w, at, p.lim, first, a.scale2);
+        if (more) wait_dma<LOADS>();                       // (the next keys' loads are younger)
+        else wait_dma<0>();
+        if (OWN && at + 32 > p.least) finite_values<E>(vs, 32 * CR, flag);
+        product<E, DP, 1>(c, vs, w);
         asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
         if (more) vals(j + NW);
     }
@@ -418,9 +429,10 @@ __device__ __forceinline__ void keys_part(const AttnArgs& a, char* lds, const Pa
         l = l * e0 + y[(DP / 2 + 1) * 64] * e1;
         c.m = mn;
 #pragma unroll
-        for (int t = 0; t < DP / 32; ++t)
+        for (int t = 0; t < DP / 32; ++t) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) c.o[t][r] = c.o[t][r] * e0 + y[(t * 16 + r) * 64] * e1;
+        }
     }
     store_part<DP, FULL>(a, c, l, p);
     if constexpr (OWN)
@@ -432,19 +444,12 @@ __device__ __forceinline__ void keys_part(const AttnArgs& a, char* lds, const Pa
 // kinds in turn, for the products of the one beside the loads of the other, takes that sharing from the
 // row tiles: 256 sequences on 131072 tokens 743 us, one kind after the other 526.)  Own: (head, row tile,
 // sequence, split).
-template <class E, int DP, bool FULL>
-__global__ __launch_bounds__(NW * 64, DP <= 128 ? 2 : 1) void segment_kernel(AttnArgs a) {
-    __shared__ __attribute__((aligned(16))) char lds[Shape<DP>::LDS + 16];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+// The part of workgroup x of its kind; `wrow`: this lane's row in a tile of bm rows; false: no key
+__device__ __forceinline__ bool find_part(const AttnArgs& a, bool own, uint32_t x, int bm, int wrow, Part& p) {
     const int R = a.Lq * a.G;
     const int64_t rows = (int64_t)a.B * a.Lq * a.Hq;
-    const bool own = blockIdx.x >= a.np;
-    uint32_t x = own ? blockIdx.x - a.np : blockIdx.x;
     const int h = x % a.Hkv;
     x /= a.Hkv;
-    const bool keys = own ? a.keys_o : a.keys_p;
-    const int wrow = (keys ? 0 : wave * 32) + (lane & 31), bm = keys ? 32 : 32 * NW;
-    Part p;
     if (!own) {
         const int M = a.B * R, tiles = (M + bm - 1) / bm;
         const int tile = x % tiles, split = x / tiles;
@@ -478,10 +483,19 @@ __global__ __launch_bounds__(NW * 64, DP <= 128 ? 2 : 1) void segment_kernel(Att
         p.at = (a.sp + split) * rows + ((int64_t)b * a.Lq + i) * a.Hq + head;
         p.sc = a.sc && p.valid ? a.sc + (((int64_t)b * a.Hkv + h) * R + mc) * a.tp : nullptr;
     }
-    if (p.key1 <= p.key0) {                                // (uniform over the workgroup)
-        if (p.valid && (keys ? wave == 0 : true) && lane < 32) { a.pm[p.at] = -__builtin_inff(); a.pl[p.at] = 0.f; }
+    if (p.key1 > p.key0) return true;                      // (uniform over the workgroup)
+    if (p.valid && (threadIdx.x & 63) < 32) { a.pm[p.at] = -__builtin_inff(); a.pl[p.at] = 0.f; }
+    return false;
+}
+
+template <class E, int DP, bool FULL>
+__global__ __launch_bounds__(NW * 64, DP <= 128 ? 2 : 1) void segment_kernel(AttnArgs a) {
+    __shared__ __attribute__((aligned(16))) char lds[Shape<DP>::LDS + 16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool own = blockIdx.x >= a.np, keys = (own ? a.rows_o : a.rows_p) == 32;
+    Part p;
+    if (!find_part(a, own, own ? blockIdx.x - a.np : blockIdx.x, keys ? 32 : 32 * NW, (keys ? 0 : wave * 32) + (lane & 31), p))
         return;
-    }
     if (!own) {
         if (keys) keys_part<E, DP, FULL, false>(a, lds, p);
         else rows_part<E, DP, FULL, false>(a, lds, p);
@@ -507,16 +521,35 @@ __global__ __launch_bounds__(256) void combine_kernel(AttnArgs a, int nw) {
         const int b = bh / a.Hkv, h = bh - b * a.Hkv;
         const int len = min(max(a.lens[b], 0), a.T);
         if (t0 >= len) return;
+        const int t = t0 + 4 * tid;
+        const float* const sc = a.sc + (int64_t)bh * R * a.tp + min(t, (int)a.tp - 4);
+        v4f s[8];                                          // eight rows' scores, on their way during the sums
+        auto load = [&](int r0) INL {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s[u] = *reinterpret_cast<const v4f*>(sc + (int64_t)min(r0 + u, R - 1) * a.tp);
+        };
+        load(0);
         // (R <= 32) a row's lse: 8 threads over its partials
         {
             const int r = min(tid >> 3, R - 1), i = r / a.G;
             const int64_t row = ((int64_t)b * a.Lq + i) * a.Hq + h * a.G + r - i * a.G;
             float m = -__builtin_inff(), l = 0.f;
-            for (int s = tid & 7; s < n; s += 8) {
-                const float m1 = a.pm[s * rows + row], l1 = a.pl[s * rows + row];
-                const float mn = fmaxf(m, m1);
-                if (mn > -__builtin_inff()) l = l * __builtin_amdgcn_exp2f(m - mn) + l1 * __builtin_amdgcn_exp2f(m1 - mn);
-                m = mn;
+            for (int k0 = tid & 7; k0 < n; k0 += 32) {
+                float ms[4], ls[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int64_t at = min(k0 + 8 * u, n - 1) * rows + row;
+                    ms[u] = a.pm[at];
+                    ls[u] = a.pl[at];
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const float mn = fmaxf(m, ms[u]);
+                    if (k0 + 8 * u < n && mn > -__builtin_inff()) {
+                        l = l * __builtin_amdgcn_exp2f(m - mn) + ls[u] * __builtin_amdgcn_exp2f(ms[u] - mn);
+                        m = mn;
+                    }
+                }
             }
 #pragma unroll
             for (int o = 1; o < 8; o <<= 1) {
@@ -527,14 +560,10 @@ __global__ __launch_bounds__(256) void combine_kernel(AttnArgs a, int nw) {
             if ((tid & 7) == 0) sm[tid >> 3] = m + __builtin_log2f(l);
         }
         __syncthreads();
-        const int t = t0 + 4 * tid;
         if (t >= len) return;
-        const float* const sc = a.sc + (int64_t)bh * R * a.tp + t;
         v4f w = {0.f, 0.f, 0.f, 0.f};
         for (int r0 = 0; r0 < R; r0 += 8) {
-            v4f s[8];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) s[u] = *reinterpret_cast<const v4f*>(sc + (int64_t)min(r0 + u, R - 1) * a.tp);
+            if (r0) load(r0);
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 const int see = r0 + u < R ? len - a.Lq + (r0 + u) / a.G : -1;   // the row's own token
@@ -672,7 +701,7 @@ __global__ __launch_bounds__(256) void weights_kernel(AttnArgs a) {
 // ---- the host's side --------------------------------------------------------------------------
 
 struct Plan {
-    bool keys_p, keys_o;                     // the workgroups' shape: prefix, own
+    int rows_p, rows_o;                      // rows of a tile: prefix, own
     int sp, ss, per_p;                       // splits; keys of a prefix split
     int64_t np, no;                          // workgroups
     int64_t rows, tp;
@@ -685,22 +714,23 @@ static Plan plan(int B, int Lq, int Hq, int Hkv, int D, int P, int T) {
     const int R = Lq * (Hq / Hkv);
     const int64_t M = (int64_t)B * R, slots = 2 * (int64_t)otpu_cu_count();
     p.rows = (int64_t)B * Lq * Hq;
-    p.keys_p = M <= 32;
-    p.keys_o = R <= 32;
-    const int64_t gp = (int64_t)Hkv * (p.keys_p ? 1 : (M + 127) / 128);
-    const int64_t go = (int64_t)B * Hkv * (p.keys_o ? 1 : (R + 127) / 128);
+    auto tile = [&](int64_t m) { return m <= 32 ? 32 : 32 * NW; };
+    p.rows_p = tile(M);
+    p.rows_o = tile(R);
+    const int64_t gp = (int64_t)Hkv * ((M + p.rows_p - 1) / p.rows_p);
+    const int64_t go = (int64_t)B * Hkv * ((R + p.rows_o - 1) / p.rows_o);
     // as many splits as fill the CUs' places, of no fewer keys than pay for a partial
     auto splits = [&](int64_t groups, int keys, int least) {
         if (keys <= 0 || groups <= 0) return 0;
         const int64_t s = (slots + groups - 1) / groups, most = (keys + least - 1) / least;
         return (int)(s > most ? most : s);
     };
-    p.sp = splits(gp, P, p.keys_p ? 128 : 512);
+    p.sp = splits(gp, P, p.rows_p == 32 ? 128 : 512);
     p.ss = splits(go, T, 256);
     p.per_p = p.sp ? ((P + p.sp - 1) / p.sp + 31) & ~31 : 0;
     p.np = gp * p.sp;
     p.no = go * p.ss;
-    p.scores = p.keys_o;
+    p.scores = p.rows_o == 32;
     p.tp = (T + 31) & ~31;
     const int64_t n = p.sp + p.ss;
     auto part = [&](int64_t floats) {
@@ -742,8 +772,7 @@ static void launch_type(const AttnArgs& a, const Plan& p, hipStream_t s) {
     else if (a.D < 64) launch_all<E, 64, false>(a, p, s);
     else if (a.D == 128) launch_all<E, 128, true>(a, p, s);
     else if (a.D < 128) launch_all<E, 128, false>(a, p, s);
-    else if (a.D == 256) launch_all<E, 256, true>(a, p, s);
-    else launch_all<E, 256, false>(a, p, s);
+    else launch_all<E, 256, false>(a, p, s);              // (256 too: the copy for whole rows spills registers)
 }
 
 }  // namespace otpu
@@ -805,7 +834,7 @@ extern "C" int otpu_attn_shared(const void* q, int64_t qb, int64_t qt, int64_t q
     a.scale2 = scale * 1.4426950408889634f;
     a.sp = p.sp; a.ss = p.ss; a.per_p = p.per_p;
     a.np = (uint32_t)p.np; a.no = (uint32_t)p.no;
-    a.keys_p = p.keys_p; a.keys_o = p.keys_o;
+    a.rows_p = p.rows_p; a.rows_o = p.rows_o;
     float* const f = (float*)work;
     a.po = f + p.po; a.pm = f + p.pm; a.pl = f + p.pl;
     a.tp = p.tp;
