@@ -94,13 +94,13 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, char* k, char* v, 
 // KPT keys a thread in registers, slots in turn over the threads; a cache of more than KPT * 1024 slots in
 // such chunks, its keys read again for each pass over them.
 template <int KPT>
-__global__ __launch_bounds__(EW, KPT <= 8 ? 8 : 4) void evict_select_kernel(EvictArgs a) {
+__global__ __launch_bounds__(EW, KPT <= 2 ? 8 : 4) void evict_select_kernel(EvictArgs a) {
     constexpr int WV = EW / 64;
     // four counts a digit, by lane: weights lie in few digits, and one address takes one lane at a time
     __shared__ __attribute__((aligned(16))) int hist[4 * BINS];
     __shared__ int2 few[HERE];               // few moves
     __shared__ int tmp[2][WV];
-    __shared__ int cnt[KPT * WV];
+    __shared__ uint64_t stay_bits[KPT * WV], tie_bits[KPT * WV];
     __shared__ uint32_t digit;
     __shared__ int above, equal;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -110,6 +110,7 @@ __global__ __launch_bounds__(EW, KPT <= 8 ? 8 : 4) void evict_select_kernel(Evic
     const int32_t* const pos = a.pos + (int64_t)bh * a.T;
     float* const wn = a.wn + (int64_t)bh * a.T;
     int32_t* const pn = a.pn + (int64_t)bh * a.T;
+    const bool new_w = wn != w, new_p = pn != pos;   // not in place
     if (tid == 0 && bh % a.H == 0 && a.ln != a.lens) a.ln[b] = left;
 
     if (n <= a.budget || a.budget == 0) {    // every slot stays, or none
@@ -147,18 +148,26 @@ __global__ __launch_bounds__(EW, KPT <= 8 ? 8 : 4) void evict_select_kernel(Evic
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < WV; ++i) newest = max(newest, tmp[0][i]);
-    const int64_t old = (int64_t)newest - a.recent;          // positions past it stay
-    // key 0: no slot (a weight's key is at least that of -inf)
-    auto keys = [&](int c) __attribute__((always_inline)) {
+    // positions from `old` on stay (none of them where recent is 0)
+    const int32_t old = (int32_t)max((int64_t)newest - a.recent + 1, (int64_t)INT32_MIN);
+    // key 0: no slot (a weight's key is at least that of -inf).  fill: what new arrays hold but for the
+    // holes, while it is at hand
+    auto keys = [&](int c, bool fill) __attribute__((always_inline)) {
         if (chunks > 1) load(c);
 #pragma unroll
         for (int i = 0; i < KPT; ++i) {
+            const int t = (c * KPT + i) * EW + tid;
             const int32_t p = HOLD ? ps[HOLD ? i : 0] : pos[slot(c, i)];
-            const uint32_t k = (int64_t)p > old ? 0xFFFFFFFFu : weight_key(HOLD ? bitsf(key[i]) : w[slot(c, i)]);
-            key[i] = (c * KPT + i) * EW + tid < n ? k : 0u;
+            const float x = HOLD ? bitsf(key[i]) : w[slot(c, i)];
+            const uint32_t k = a.recent > 0 && p >= old ? 0xFFFFFFFFu : weight_key(x);
+            key[i] = t < n ? k : 0u;
+            if (fill && t < left) {
+                if (new_w) wn[t] = x;
+                if (new_p) pn[t] = p;
+            }
         }
     };
-    if (chunks == 1) keys(0);
+    if (chunks == 1) keys(0, true);
 
     // the key of the left-th slot, and how many of the slots with that key stay
     uint32_t prefix = 0, mask = 0;
@@ -169,7 +178,7 @@ __global__ __launch_bounds__(EW, KPT <= 8 ? 8 : 4) void evict_select_kernel(Evic
         const uint32_t dm = pass == 2 ? 0x3FFu : 0x7FFu;
 #pragma unroll 1
         for (int c = 0; c < chunks; ++c) {
-            if (chunks > 1) keys(c);
+            if (chunks > 1) keys(c, pass == 0);
 #pragma unroll
             for (int i = 0; i < KPT; ++i)      // (key 0 is below every slot's: never chosen)
                 if ((key[i] & mask) == prefix) atomicAdd(&hist[4 * ((key[i] >> shift) & dm) + (lane & 3)], 1);
@@ -196,67 +205,45 @@ __global__ __launch_bounds__(EW, KPT <= 8 ? 8 : 4) void evict_select_kernel(Evic
         if (same == need) break;              // (uniform) all of this digit's slots stay: no ties
     }
 
-    // in slot order: which of the equal keys stay, the holes and the sources.  cnt: a wave's count at each of
-    // its KPT places, summed in slot order
+    // In slot order: which of the equal keys stay, the holes and the sources.  A wave's slots at one place are
+    // 64 in a row, so the ballots of a comparison, place after place and wave after wave, are its bits in slot
+    // order, and a thread goes on with 32 of them.
     int2* const mv = a.here ? few : a.moves + (int64_t)bh * a.most;
-    int ties = 0, holes = 0, extras = 0;
-    const uint64_t below = (1ull << lane) - 1;
-    auto ordered = [&]() __attribute__((always_inline)) {    // cnt: exclusive sums; returns the whole sum
-        __syncthreads();
-        const int mine = tid < KPT * WV ? cnt[tid] : 0;
-        int total;
-        const int x = block_scan(mine, tmp[0], total);
-        if (tid < KPT * WV) cnt[tid] = x;
-        __syncthreads();
-        return total;
-    };
+    int ties = 0, holes = 0, extras = 0, total;
 #pragma unroll 1
     for (int c = 0; c < chunks; ++c) {
-        if (chunks > 1) keys(c);
-        uint32_t stay = 0;                                   // bit i: the slot at place i stays
-        if (same == need) {
+        if (chunks > 1) keys(c, false);
+        __syncthreads();
 #pragma unroll
-            for (int i = 0; i < KPT; ++i) stay |= (uint32_t)(key[i] >= prefix) << i;
-        } else {
-#pragma unroll
-            for (int i = 0; i < KPT; ++i) {
-                const int v = __builtin_popcountll(__ballot(key[i] == prefix));
-                if (lane == 0) cnt[i * WV + wave] = v;
-            }
-            const int total = ordered();
+        for (int i = 0; i < KPT; ++i) {
+            const uint64_t above_it = __ballot(key[i] > prefix || (same == need && key[i] >= prefix));
+            if (lane == 0) stay_bits[i * WV + wave] = above_it;
+        }
+        if (same != need) {
 #pragma unroll
             for (int i = 0; i < KPT; ++i) {
-                const bool tie = key[i] == prefix;
-                const int rank = ties + cnt[i * WV + wave] + __builtin_popcountll(__ballot(tie) & below);
-                stay |= (uint32_t)(key[i] > prefix || (tie && rank < need)) << i;
+                const uint64_t tie = __ballot(key[i] == prefix);
+                if (lane == 0) tie_bits[i * WV + wave] = tie;
             }
+        }
+        __syncthreads();
+        const bool mine = tid < KPT * 32;
+        uint32_t stay = mine ? reinterpret_cast<const uint32_t*>(stay_bits)[tid] : 0u;
+        if (same != need) {
+            uint32_t tie = mine ? reinterpret_cast<const uint32_t*>(tie_bits)[tid] : 0u;
+            int room = need - ties - block_scan(__builtin_popcount(tie), tmp[0], total);
             ties += total;
+            for (; tie && room > 0; --room, tie &= tie - 1) stay |= tie & -tie;
             __syncthreads();
         }
-        // a slot below `left` that goes, or one at or past it that stays
-        int t0 = c * KPT * EW + tid;
-        // (both as values in a register: a mask a slot, kept over the barriers, takes more scalar ones than
-        // there are)
-        asm volatile("" : "+v"(stay));
-#pragma unroll
-        for (int i = 0; i < KPT; ++i) {
-            const bool s = (stay >> i) & 1, low = t0 + i * EW < left;
-            const int v = __builtin_popcountll(__ballot(low && !s)) | __builtin_popcountll(__ballot(!low && s)) << 16;
-            if (lane == 0) cnt[i * WV + wave] = v;
-        }
-        const int total = ordered();
-        asm volatile("" : "+v"(stay), "+v"(t0));
-#pragma unroll
-        for (int i = 0; i < KPT; ++i) {
-            const int t = t0 + i * EW, at = cnt[i * WV + wave];
-            const bool s = (stay >> i) & 1, low = t < left;
-            const uint64_t holes_of = __ballot(low && !s), extras_of = __ballot(!low && s);
-            if (low && !s) mv[holes + (at & 0xFFFF) + __builtin_popcountll(holes_of & below)].x = t;
-            if (!low && s) mv[extras + (at >> 16) + __builtin_popcountll(extras_of & below)].y = t;
-            if (low && s && wn != w) { wn[t] = w[t]; pn[t] = pos[t]; }
-        }
+        const int t0 = (c * KPT * 32 + tid) * 32;            // this thread's first slot
+        const uint32_t low = !mine || t0 >= left ? 0u : (left - t0 >= 32 ? ~0u : (1u << (left - t0)) - 1);
+        uint32_t hole = low & ~stay, extra = mine ? stay & ~low : 0u;
+        const uint32_t at = (uint32_t)block_scan(__builtin_popcount(hole) | __builtin_popcount(extra) << 16, tmp[1], total);
+        for (int j = holes + (int)(at & 0xFFFF); hole; ++j, hole &= hole - 1) mv[j].x = t0 + __builtin_ctz(hole);
+        for (int j = extras + (int)(at >> 16); extra; ++j, extra &= extra - 1) mv[j].y = t0 + __builtin_ctz(extra);
         holes += total & 0xFFFF;
-        extras += total >> 16;
+        extras += (int)((uint32_t)total >> 16);
     }
     __syncthreads();
     for (int j = tid; j < holes; j += EW) {
@@ -265,7 +252,7 @@ __global__ __launch_bounds__(EW, KPT <= 8 ? 8 : 4) void evict_select_kernel(Evic
         pn[m.x] = pos[m.y];
     }
     if (a.here) move_rows<EW, 1>(a, a.k + b * a.kb + (bh - b * a.H) * a.kh, a.v + b * a.vb + (bh - b * a.H) * a.vh, mv, holes, 0, 1);
-    __syncthreads();
+    __syncthreads();                          // the sources are read, in place too
     for (int t = left + tid; t < a.T; t += EW) { wn[t] = 0.f; pn[t] = -1; }
     if (tid == 0) a.count[bh] = holes;
 }

@@ -108,6 +108,22 @@ def test_strides_types_and_lengths_out_of_range(T):
         assert np.array_equal(g.cpu().numpy(), x)
 
 
+def test_some_in_place(T):
+    """Each of the three outputs in place or not by itself."""
+    from opentpu_amd import attention
+    rng = np.random.default_rng(6)
+    B, Tn, H, D, budget = 2, 1500, 2, 16, 700
+    k, v, w, pos, lens = make(rng, B, Tn, H, D, budget, "ties")
+    want = reference(k, v, w, pos, lens, budget, 9)
+    for which in range(8):
+        kd, vd = (T.from_numpy(x).cuda().view(T.bfloat16) for x in (k, v))
+        old = [T.from_numpy(x).cuda() for x in (w, pos, lens)]
+        out = [x if which >> i & 1 else T.full_like(x, 77) for i, x in enumerate(old)]
+        attention.evict(kd, vd, *old, budget, 9, out=out)
+        for g, x in zip((kd.view(T.int16), vd.view(T.int16), *out), want):
+            assert np.array_equal(g.cpu().numpy(), x), which
+
+
 def test_graph(T):
     """Captured, and replayed on caches filled anew, eager work between."""
     from opentpu_amd import attention
