@@ -99,7 +99,7 @@ def shared(q, prefix_k, prefix_v, k, v, lens, *, scale: float | None = None, wei
     if out.numel() == 0:
         return out
     nbytes = _attn_bytes(B, Lq, Hq, Hkv, D, P, N)
-    work = T.empty((max(nbytes, 1),), dtype=T.uint8, device=q.device)
+    work = q.new_empty((nbytes // 2 + 1,))                 # (of q's type: the least work for the host)
     X.call("otpu_attn_shared", q.data_ptr(), qs[0], qs[1], qs[2], pk, ps[0], ps[1], pv, pvs[0], pvs[1], P, kp, ks[0],
            ks[1], ks[2], vp, vs[0], vs[1], vs[2], lp, N, B, Lq, Hq, Hkv, D, kinds[dt],
            D ** -0.5 if scale is None else scale, out.data_ptr(), os[0], os[1], os[2], wp, work.data_ptr(), nbytes,
@@ -131,7 +131,7 @@ def evict(k, v, weights, pos, lens, budget: int, recent: int = 0, *, out=None):
     new = (_dense("evict", "out[0]", out[0], T.float32, slots, dev), _dense("evict", "out[1]", out[1], T.int32, slots, dev),
            _dense("evict", "out[2]", out[2], T.int32, (B,), dev))
     nbytes = _evict_bytes(B, N, H, budget)
-    work = T.empty((max(nbytes, 1),), dtype=T.uint8, device=k.device)
+    work = lens.new_empty((nbytes // 4 + 1,))
     X.call("otpu_kv_evict", k.data_ptr(), e * ks[0], e * ks[1], e * ks[2], v.data_ptr(), e * vs[0], e * vs[1], e * vs[2],
            e * D, *old, B, N, H, budget, recent, *new, work.data_ptr(), nbytes, X.stream())
     return out

@@ -97,7 +97,7 @@ template <int DP_> struct Shape {
     static constexpr int RB = KT * DP * 2;                 // ... their bytes, and their values'
     static constexpr int KB = 32 * DP * 2;                 // keys: a wave's keys' bytes, and its values'
     static constexpr int MERGE = (NW - 1) * 64 * (DP / 2 + 2) * 4;
-    static constexpr int ROWS_LDS = 4 * RB, KEYS_LDS = NW * 2 * KB > MERGE ? NW * 2 * KB : MERGE;
+    static constexpr int ROWS_LDS = 4 * RB, KEYS_LDS = NW * 2 * KB > MERGE + 4 ? NW * 2 * KB : MERGE + 4;
     static constexpr int LDS = ROWS_LDS > KEYS_LDS ? ROWS_LDS : KEYS_LDS;
 };
 
@@ -141,10 +141,11 @@ template <int DP> struct Acc {
 };
 
 // An infinity or NaN among the values of a key that some row does not see would reach that row as
-// 0 * inf.  So a step with such keys multiplies the finite values alone (the others are set to zero, and
-// the flag), and add_infinite adds the others to the partials of the rows that see them.
+// 0 * inf.  So a step with such keys multiplies the finite values alone (the others are set to zero, which
+// the result says), and add_infinite adds the others to the partials of the rows that see them.
 template <class E>
-__device__ __forceinline__ void finite_values(char* vs, int pieces, int* flag) {
+__device__ __forceinline__ bool finite_values(char* vs, int pieces) {
+    bool found = false;
     constexpr uint32_t EX = E::INF * 0x10001u, LO = (0x8000u - E::INF) * 0x10001u;
 #pragma unroll 1
     for (int x = threadIdx.x & 63; x < pieces; x += 64) {
@@ -153,9 +154,10 @@ __device__ __forceinline__ void finite_values(char* vs, int pieces, int* flag) {
         if ((bad[0] | bad[1] | bad[2] | bad[3]) != 0) {
             w &= ~((bad >> 15) * 0xFFFFu);
             reinterpret_cast<v4u*>(vs)[x] = w;
-            *flag = 1;
+            found = true;
         }
     }
+    return __any(found);
 }
 
 // S^T = K Q^T of 32 TT keys at ks (LDS): a lane has its row's scores of keys 8 r + 4 hh + 0..3 of each 32
@@ -308,6 +310,17 @@ __device__ __forceinline__ void add_infinite(const AttnArgs& a, const Part& p) {
     }
 }
 
+// whether `x` holds in a wave of the workgroup; at: a word of LDS that no wave needs any more
+__device__ __forceinline__ bool any_wave(char* at, bool x) {
+    int* const word = reinterpret_cast<int*>(at);
+    bar();
+    *word = 0;
+    bar();
+    if (x) *word = 1;
+    bar();
+    return __builtin_amdgcn_readfirstlane(*word) != 0;
+}
+
 __device__ __forceinline__ int wave_min(int x) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) x = min(x, __shfl_xor(x, o, 64));   // (both halves hold the same rows)
@@ -327,8 +340,6 @@ __device__ __forceinline__ void rows_part(const AttnArgs& a, char* lds, const Pa
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Acc<DP> c;
     c.clear();
-    int* const flag = reinterpret_cast<int*>(lds + S::LDS);
-    if (OWN) *flag = 0;                                    // (every thread; a barrier follows)
     if (!FULL) clear_lds(lds, S::ROWS_LDS);
     v8s qf[DP / 16];
     load_query<DP, FULL>(qf, p.q, a.D);
@@ -341,6 +352,7 @@ __device__ __forceinline__ void rows_part(const AttnArgs& a, char* lds, const Pa
     };
     issue(0);
     const int first = wave_min(p.lim), none = -wave_min(-p.lim);
+    bool bad = false;
     for (int i = 0; i < steps; ++i) {
         wait_dma<0>();
         bar();
@@ -352,14 +364,12 @@ __device__ __forceinline__ void rows_part(const AttnArgs& a, char* lds, const Pa
         v8s w[KT / 16];
         scores<E, DP>(s, ks, qf);
         softmax<E>(c, s, w, at, p.lim, first, a.scale2);
-        if (OWN && at + KT > p.least) finite_values<E>(ks + S::RB, KT * CR, flag);
+        if (OWN && at + KT > p.least) bad |= finite_values<E>(ks + S::RB, KT * CR);
         product<E, DP, KT / 32>(c, ks + S::RB, w);
     }
     store_part<DP, FULL>(a, c, swap32_sum(c.l), p);
-    if constexpr (OWN) {
-        bar();
-        if (*flag) add_infinite<E, KT>(a, p);
-    }
+    if constexpr (OWN)
+        if (any_wave(lds, bad)) add_infinite<E, KT>(a, p);
 }
 
 template <class E, int DP, bool FULL, bool OWN>
@@ -369,8 +379,6 @@ __device__ __forceinline__ void keys_part(const AttnArgs& a, char* lds, const Pa
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Acc<DP> c;
     c.clear();
-    int* const flag = reinterpret_cast<int*>(lds + S::LDS);
-    if (OWN) { *flag = 0; bar(); }                         // (no other barrier before the last)
     if (!FULL) clear_lds(lds, S::KEYS_LDS);
     char* const ks = lds + wave * 2 * S::KB;
     char* const vs = ks + S::KB;
@@ -381,6 +389,7 @@ __device__ __forceinline__ void keys_part(const AttnArgs& a, char* lds, const Pa
     v8s qf[DP / 16];
     load_query<DP, FULL>(qf, p.q, a.D);
     const int first = wave_min(p.lim);
+    bool bad = false;
     if (wave < tiles) { keys(wave); vals(wave); }
     for (int j = wave; j < tiles; j += NW) {
         const bool more = j + NW < tiles;
@@ -400,7 +409,7 @@ __device__ __forceinline__ void keys_part(const AttnArgs& a, char* lds, const Pa
         softmax<E>(c, s, w, at, p.lim, first, a.scale2);
         if (more) wait_dma<LOADS>();                       // (the next keys' loads are younger)
         else wait_dma<0>();
-        if (OWN && at + 32 > p.least) finite_values<E>(vs, 32 * CR, flag);
+        if (OWN && at + 32 > p.least) bad |= finite_values<E>(vs, 32 * CR);
         product<E, DP, 1>(c, vs, w);
         asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
         if (more) vals(j + NW);
@@ -420,6 +429,7 @@ __device__ __forceinline__ void keys_part(const AttnArgs& a, char* lds, const Pa
         y[(DP / 2 + 1) * 64] = l;
     }
     bar();
+    const bool any_bad = OWN && any_wave(lds + S::MERGE, bad);
     if (wave > 0) return;
     for (int w = 0; w < NW - 1 && w + 1 < tiles; ++w) {
         const float* const y = x + w * ST * 64 + lane;
@@ -436,7 +446,7 @@ __device__ __forceinline__ void keys_part(const AttnArgs& a, char* lds, const Pa
     }
     store_part<DP, FULL>(a, c, l, p);
     if constexpr (OWN)
-        if (*flag) add_infinite<E, 32>(a, p);
+        if (any_bad) add_infinite<E, 32>(a, p);
 }
 
 // The workgroups of the prefix, then those of the own keys.  Prefix: (head, row tile, split), the heads over
@@ -490,7 +500,7 @@ __device__ __forceinline__ bool find_part(const AttnArgs& a, bool own, uint32_t 
 
 template <class E, int DP, bool FULL>
 __global__ __launch_bounds__(NW * 64, DP <= 128 ? 2 : 1) void segment_kernel(AttnArgs a) {
-    __shared__ __attribute__((aligned(16))) char lds[Shape<DP>::LDS + 16];
+    __shared__ __attribute__((aligned(16))) char lds[Shape<DP>::LDS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool own = blockIdx.x >= a.np, keys = (own ? a.rows_o : a.rows_p) == 32;
     Part p;
@@ -581,8 +591,13 @@ __global__ __launch_bounds__(256) void combine_kernel(AttnArgs a, int nw) {
     }
     const int per = a.D / 4, rpb = 256 / (per * GP);       // rows a workgroup
     const int rl = tid / (per * GP), y = tid - rl * per * GP, g = y / per, d = (y - g * per) * 4;
-    const int64_t row = (int64_t)(blockIdx.x - nw) * rpb + rl;
-    const bool ok = rl < rpb && row < rows;
+    // rows of one head of the keys, on the XCD whose L2 its partials were written through
+    const int x = blockIdx.x - nw, hk = x % a.Hkv, R = a.Lq * a.G;
+    const int64_t mr = (int64_t)(x / a.Hkv) * rpb + rl;    // (b, i, g)
+    const bool ok = rl < rpb && mr < (int64_t)a.B * R;
+    const int64_t bi = mr / a.G;
+    const int head = hk * a.G + (int)(mr - bi * a.G);
+    const int64_t row = bi * a.Hq + head;
     float m = -__builtin_inff(), l = 0.f;
     v4f o = {0.f, 0.f, 0.f, 0.f};
     if (ok) {
@@ -639,10 +654,8 @@ __global__ __launch_bounds__(256) void combine_kernel(AttnArgs a, int nw) {
     typename E::v4 z;
 #pragma unroll
     for (int j = 0; j < 4; ++j) z[j] = (typename E::e)(o[j] * il);
-    const int head = (int)(row % a.Hq);
-    const int64_t bi = row / a.Hq;
-    const int i = (int)(bi % a.Lq);
     const int64_t b = bi / a.Lq;
+    const int i = (int)(bi - b * a.Lq);
     *reinterpret_cast<typename E::v4*>(a.out + b * a.ob + i * a.ot + head * a.oh + d * 2) = z;
     if (a.lse && d == 0) a.lse[row] = m + __builtin_log2f(l);
 }
@@ -719,17 +732,27 @@ static Plan plan(int B, int Lq, int Hq, int Hkv, int D, int P, int T) {
     p.rows_o = tile(R);
     const int64_t gp = (int64_t)Hkv * ((M + p.rows_p - 1) / p.rows_p);
     const int64_t go = (int64_t)B * Hkv * ((R + p.rows_o - 1) / p.rows_o);
-    // as many splits as fill the CUs' places, of no fewer keys than pay for a partial
-    auto splits = [&](int64_t groups, int keys, int least) {
-        if (keys <= 0 || groups <= 0) return 0;
+    // Splits: as many as fill the places of the CUs, of `least` keys or more.
+    auto splits = [&](int64_t groups, int64_t keys, int64_t least) {
+        if (keys <= 0 || groups <= 0) return (int64_t)0;
         const int64_t s = (slots + groups - 1) / groups, most = (keys + least - 1) / least;
-        return (int)(s > most ? most : s);
+        return s > most ? most : s;
     };
-    p.sp = splits(gp, P, p.rows_p == 32 ? 128 : 512);
-    p.ss = splits(go, T, 256);
+    p.ss = (int)splits(go, T, 256);
+    p.no = go * p.ss;
+    int64_t s = splits(gp, P, p.rows_p == 32 ? 128 : 64);
+    if (p.rows_p > 32 && s > 1) {
+        // A tile of 128 rows writes 64 KB of partials a split, read once more, where another split saves
+        // each workgroup steps: the sum is least near sqrt(P / (2 groups)) (64 sequences on 4096 tokens, 8
+        // groups: 8, 16 and 32 splits 18.6, 15.1 and 17.3 us; on 16384 16, 32 and 64 33.6, 28.3 and 31.2).
+        // Half of that beside own keys that fill the CUs: there the steps' latency does not count (64
+        // sequences on 16384, up to 1024 own tokens: 32 splits 64 us, 16 59, 8 80).
+        const int64_t r = (int64_t)__builtin_ceil(__builtin_sqrt((double)P / (2.0 * (double)gp)));
+        if (r < s) s = p.no >= slots / 2 ? (r + 1) / 2 : r;
+    }
+    p.sp = (int)s;
     p.per_p = p.sp ? ((P + p.sp - 1) / p.sp + 31) & ~31 : 0;
     p.np = gp * p.sp;
-    p.no = go * p.ss;
     p.scores = p.rows_o == 32;
     p.tp = (T + 31) & ~31;
     const int64_t n = p.sp + p.ss;
@@ -749,7 +772,7 @@ static Plan plan(int B, int Lq, int Hq, int Hkv, int D, int P, int T) {
 template <class E, int GP>
 static void launch_combine(const AttnArgs& a, const Plan& p, hipStream_t s) {
     const int rpb = 256 / (a.D / 4 * GP);
-    const int nrows = (int)((p.rows + rpb - 1) / rpb);
+    const int nrows = a.Hkv * (int)(((int64_t)a.B * a.Lq * a.G + rpb - 1) / rpb);
     const int nw = a.sc ? a.B * a.Hkv * ((a.T + WT - 1) / WT) : 0;
     combine_kernel<E, GP><<<nrows + nw, 256, 0, s>>>(a, nw);
 }
@@ -759,8 +782,8 @@ static void launch_all(const AttnArgs& a, const Plan& p, hipStream_t s) {
     if (p.np + p.no) segment_kernel<E, DP, FULL><<<(unsigned)(p.np + p.no), NW * 64, 0, s>>>(a);
     // threads a partial's row: by how many partials there are (at most 256 in all: D / 4 columns' threads)
     const int n = p.sp + p.ss;
-    if (n > 8 && a.D <= 128) launch_combine<E, 8>(a, p, s);
-    else if (n > 4) launch_combine<E, 4>(a, p, s);
+    if (n > 8) launch_combine<E, 4>(a, p, s);
+    else if (n > 2) launch_combine<E, 2>(a, p, s);
     else launch_combine<E, 1>(a, p, s);
     if (a.weights && a.T && !a.sc)
         weights_kernel<E, DP, FULL><<<(unsigned)((int64_t)a.B * a.Hkv * ((a.T + 127) / 128)), 256, 0, s>>>(a);

@@ -240,8 +240,8 @@ def norm_quantize(x, gamma, residual=None, *, eps: float = 1e-6, row_mode: bool 
     if r is not None and (r.dtype != T.float32 or r.shape != (M,) or not r.is_contiguous() or r.get_device() != dev):
         raise ValueError("norm_quantize: r is a contiguous float32 tensor [M]")
     q = T.empty_like(x, dtype=T.int8, memory_format=T.contiguous_format)
-    S = T.empty((1, M), dtype=T.float32, device=x.device)
-    d = T.empty((M, K // 32), dtype=T.uint8, device=x.device)
+    S = gamma.new_empty((1, M))
+    d = q.new_empty((M, K // 32), dtype=T.uint8)
     X.call("otpu_norm_qact", *xp, *rp, NORM_TYPES[dt], M, K, gamma.data_ptr(), eps, X.Q_ROW if row_mode else 0, *hp,
            None if r is None else r.data_ptr(), q.data_ptr(), K, S.data_ptr(), d.data_ptr(), K // 32, X.stream())
     return _operand(q, S, d, [K], bool(row_mode)), x if h is None else h
