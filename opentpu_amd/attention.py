@@ -45,10 +45,12 @@ def _dense(who: str, name: str, t, dtype, shape, dev: int) -> int:
     return t.data_ptr()
 
 
-def _rows(who: str, name: str, t, dtype, shape, dev: int) -> tuple:
-    """The strides of a tensor whose columns are adjacent."""
+def _rows(who: str, name: str, t, dtype, shape, dev: int, written: bool = False) -> tuple:
+    """The strides of a tensor whose columns are adjacent (written: and which is no broadcast one)."""
     _check(who, name, t, dtype, shape, dev)
     s = t.stride()
+    if written and 0 in s and any(n > 1 and not x for n, x in zip(shape, s)):
+        raise ValueError(f"{who}: {name} is a broadcast tensor, it cannot be written to")
     if s[-1] != 1 and t.numel() and shape[-1] > 1:
         raise ValueError(f"{who}: the columns of {name} must be adjacent")
     return s
@@ -95,7 +97,7 @@ def shared(q, prefix_k, prefix_v, k, v, lens, *, scale: float | None = None, wei
         wp = _dense("shared", "weights", weights, T.float32, (B, Hkv, N), dev)
     if out is None:
         out = T.empty_like(q, memory_format=T.contiguous_format)
-    os = _rows("shared", "out", out, dt, (B, Lq, Hq, D), dev)
+    os = _rows("shared", "out", out, dt, (B, Lq, Hq, D), dev, True)
     if out.numel() == 0:
         return out
     nbytes = _attn_bytes(B, Lq, Hq, Hkv, D, P, N)
@@ -122,7 +124,7 @@ def evict(k, v, weights, pos, lens, budget: int, recent: int = 0, *, out=None):
         raise ValueError(f"evict: k is {dt} {list(k.shape)} on {k.device}, needs [B, T, H, D] in bfloat16, float16 or float32")
     B, N, H, D = k.shape
     e = k.element_size()
-    ks, vs = _rows("evict", "k", k, dt, (B, N, H, D), dev), _rows("evict", "v", v, dt, (B, N, H, D), dev)
+    ks, vs = _rows("evict", "k", k, dt, (B, N, H, D), dev, True), _rows("evict", "v", v, dt, (B, N, H, D), dev, True)
     slots = (B, H, N)
     old = (_dense("evict", "weights", weights, T.float32, slots, dev), _dense("evict", "pos", pos, T.int32, slots, dev),
            _dense("evict", "lens", lens, T.int32, (B,), dev))

@@ -236,6 +236,8 @@ def norm_quantize(x, gamma, residual=None, *, eps: float = 1e-6, row_mode: bool 
         raise ValueError(f"norm_quantize: gamma {list(gamma.shape)} over {K} columns")
     if h is None and residual is not None:
         h = T.empty_like(x, memory_format=T.contiguous_format)
+    if h is not None and M > 1 and h.stride(0) == 0:
+        raise ValueError("norm_quantize: h is a broadcast tensor, it cannot be written to")
     xp, rp, hp = row("x", x), (None, 0) if residual is None else row("residual", residual), (None, 0) if h is None else row("h", h)
     if r is not None and (r.dtype != T.float32 or r.shape != (M,) or not r.is_contiguous() or r.get_device() != dev):
         raise ValueError("norm_quantize: r is a contiguous float32 tensor [M]")

@@ -206,6 +206,17 @@ def test_long_prefix_past_32_bits(T):
     assert T.equal(got, attention.shared(q, pk, pv, k, v, lens))
 
 
+def test_broadcast_inputs(T):
+    """One query row, one prefix and one cache for all, as expanded tensors."""
+    from opentpu_amd import attention
+    rng = np.random.default_rng(11)
+    q, pk, pv, k, v, lens = (t.cuda() for t in make(T, rng, T.float16, 1, 1, 2, 1, 64, 30, 20))
+    B = 5
+    args = [q.expand(B, 3, 2, 64), pk.expand(30, 2, 64), pv.expand(30, 2, 64), k.expand(B, 20, 2, 64), v.expand(B, 20, 2, 64),
+            T.arange(B, dtype=T.int32, device="cuda")]
+    assert T.equal(attention.shared(*args), attention.shared(*(t.contiguous() for t in args)))
+
+
 def test_stream_and_graph(T):
     """On another stream than the default one, and captured: replays with new inputs, eager work between."""
     from opentpu_amd import attention
@@ -247,6 +258,7 @@ def test_no_queries_and_refusals(T):
                 lambda: attention.shared(q, pk, pv, k, v, lens, weights=T.zeros((2, 2, 9), device="cuda")),
                 lambda: attention.shared(q, pk, pv, k, v, lens, weights=T.zeros((2, 10, 2), device="cuda").transpose(1, 2)),
                 lambda: attention.shared(q, pk, pv, k, v, lens, out=T.empty_like(q[:1])),
+                lambda: attention.shared(q, pk, pv, k, v, lens, out=T.empty_like(q[:1]).expand_as(q)),
                 lambda: attention.shared(q.transpose(2, 3), pk, pv, k, v, lens),
                 lambda: attention.shared(q.cpu(), pk, pv, k, v, lens), lambda: attention.shared(q, pk.cpu(), pv, k, v, lens)):
         with pytest.raises(ValueError):

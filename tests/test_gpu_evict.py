@@ -158,7 +158,7 @@ def test_refusals(T):
                 lambda: attention.evict(k, v.half(), w, pos, lens, 9), lambda: attention.evict(k, v, w.double(), pos, lens, 9),
                 lambda: attention.evict(k, v, w, pos.long(), lens, 9), lambda: attention.evict(k, v, w[:, :1], pos, lens, 9),
                 lambda: attention.evict(k, v, w, pos, lens[:1], 9), lambda: attention.evict(k, v[:, :20], w, pos, lens, 9),
-                lambda: attention.evict(k.cpu(), v, w, pos, lens, 9),
+                lambda: attention.evict(k[:1].expand_as(k), v, w, pos, lens, 9), lambda: attention.evict(k.cpu(), v, w, pos, lens, 9),
                 lambda: attention.evict(k, v, w.transpose(1, 2).contiguous().transpose(1, 2), pos, lens, 9),
                 lambda: attention.evict(k, v, w, pos, lens, 9, out=(w, pos, lens[:1]))):
         with pytest.raises(ValueError):

@@ -114,7 +114,7 @@ def test_refusals(T):
     for bad in (lambda: mxu.norm_quantize(x.double(), g), lambda: mxu.norm_quantize(x[0], g),
                 lambda: mxu.norm_quantize(x, g[:128]), lambda: mxu.norm_quantize(x, g, x.half()),
                 lambda: mxu.norm_quantize(x, g, x[:2]), lambda: mxu.norm_quantize(x, g, x, h=x[:2]),
-                lambda: mxu.norm_quantize(x, g, x, h=x.half()), lambda: mxu.norm_quantize(x, g, r=g[:3]),
+                lambda: mxu.norm_quantize(x, g, x, h=x.half()), lambda: mxu.norm_quantize(x, g, x, h=x[:1].expand(4, 256)), lambda: mxu.norm_quantize(x, g, r=g[:3]),
                 lambda: mxu.norm_quantize(x.T, g[:4]), lambda: mxu.norm_quantize(x.cpu(), g)):
         with pytest.raises(ValueError):
             bad()
