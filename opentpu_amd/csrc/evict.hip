@@ -40,27 +40,30 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return (u >> 31) ? ~u : (u | 0x80000000u);
 }
 
+// inclusive sums over 16 lanes of a row, and over the wave (DPP row_shr 1, 2, 4, 8, row_bcast 15 and 31)
+__device__ __forceinline__ int row_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
+    return x + __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
+}
+__device__ __forceinline__ int wave_scan(int x) {
+    x = row_scan(x);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
+    return x + __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
+}
+
 // exclusive sum of v over the workgroup's threads, in thread order; total: the whole sum.  tmp: EW / 64
-// words that the next call does not use
+// words that the next call does not use.  Every lane of every wave takes part.
+static_assert(EW / 64 == 16, "the waves' sums in a row of 16 lanes");
 __device__ __forceinline__ int block_scan(int v, int* tmp, int& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int x = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o, 64);
-        if (lane >= o) x += y;
-    }
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int x = wave_scan(v);
     if (lane == 63) tmp[wave] = x;
     __syncthreads();
-    int before = 0, all = 0;
-#pragma unroll
-    for (int i = 0; i < EW / 64; ++i) {
-        const int t = tmp[i];
-        before += i < wave ? t : 0;
-        all += t;
-    }
-    total = all;
-    return before + x - v;
+    const int y = row_scan(tmp[lane & 15]);
+    total = __builtin_amdgcn_readlane(y, 15);
+    return (wave ? __builtin_amdgcn_readlane(y, wave - 1) : 0) + x - v;
 }
 
 // rows of k and v from slot m.y to slot m.x, `c` pieces of 16 bytes each: threads in groups of c (or all of
@@ -125,29 +128,29 @@ __global__ __launch_bounds__(EW, KPT <= 2 ? 8 : 4) void evict_select_kernel(Evic
     const int chunks = (n + EW * KPT - 1) / (EW * KPT);
     uint32_t key[KPT];
     int32_t newest = INT32_MIN;              // the newest position
-    // positions and weights come in one trip where registers hold both, else the positions twice
-    constexpr bool HOLD = KPT <= 16;
-    int32_t ps[HOLD ? KPT : 1];
-    auto slot = [&](int c, int i) __attribute__((always_inline)) { return min((c * KPT + i) * EW + tid, n - 1); };
+    int32_t ps[KPT];
+    const uint32_t utid = tid;               // (uniform addresses and this offset: few registers)
     auto load = [&](int c) __attribute__((always_inline)) {
-        if constexpr (HOLD) {
 #pragma unroll
-            for (int i = 0; i < KPT; ++i) ps[i] = pos[slot(c, i)];
-#pragma unroll
-            for (int i = 0; i < KPT; ++i) key[i] = fbits(w[slot(c, i)]);
+        for (int i = 0; i < KPT; ++i) {
+            const int t0 = (c * KPT + i) * EW;
+            ps[i] = INT32_MIN;
+            key[i] = 0;
+            if (t0 + tid < n) {
+                ps[i] = (pos + t0)[utid];
+                key[i] = fbits((w + t0)[utid]);
+            }
         }
     };
     for (int c = 0; c < chunks; ++c) {
         load(c);
 #pragma unroll
-        for (int i = 0; i < KPT; ++i) newest = max(newest, HOLD ? ps[HOLD ? i : 0] : pos[slot(c, i)]);
+        for (int i = 0; i < KPT; ++i) newest = max(newest, ps[i]);
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) newest = max(newest, __shfl_xor(newest, o, 64));
-    if (lane == 0) tmp[0][wave] = newest;
+    const uint32_t top = wave_max_dpp((uint32_t)newest ^ 0x80000000u, 64);
+    if (lane == 0) tmp[0][wave] = (int)top;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < WV; ++i) newest = max(newest, tmp[0][i]);
+    newest = (int32_t)(wave_max_dpp((uint32_t)tmp[0][lane & 15], 16) ^ 0x80000000u);
     // positions from `old` on stay (none of them where recent is 0)
     const int32_t old = (int32_t)max((int64_t)newest - a.recent + 1, (int64_t)INT32_MIN);
     // key 0: no slot (a weight's key is at least that of -inf).  fill: what new arrays hold but for the
@@ -156,15 +159,13 @@ __global__ __launch_bounds__(EW, KPT <= 2 ? 8 : 4) void evict_select_kernel(Evic
         if (chunks > 1) load(c);
 #pragma unroll
         for (int i = 0; i < KPT; ++i) {
-            const int t = (c * KPT + i) * EW + tid;
-            const int32_t p = HOLD ? ps[HOLD ? i : 0] : pos[slot(c, i)];
-            const float x = HOLD ? bitsf(key[i]) : w[slot(c, i)];
-            const uint32_t k = a.recent > 0 && p >= old ? 0xFFFFFFFFu : weight_key(x);
-            key[i] = t < n ? k : 0u;
+            const int t0 = (c * KPT + i) * EW, t = t0 + tid;
+            const uint32_t k = a.recent > 0 && ps[i] >= old ? 0xFFFFFFFFu : weight_key(bitsf(key[i]));
             if (fill && t < left) {
-                if (new_w) wn[t] = x;
-                if (new_p) pn[t] = p;
+                if (new_w) (wn + t0)[utid] = bitsf(key[i]);
+                if (new_p) (pn + t0)[utid] = ps[i];
             }
+            key[i] = t < n ? k : 0u;
         }
     };
     if (chunks == 1) keys(0, true);
