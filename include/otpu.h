@@ -403,14 +403,24 @@ int otpu_norm_qact(const void* x, int64_t ldx, const void* res, int64_t ldr, int
  *   query heads, are added to it.  dtype OTPU_BF16 or OTPU_F16 for q, caches and out; sums, maxima and
  *   weights fp32.  D a multiple of 8, at most 256; scale > 0; addresses 16-byte aligned, strides
  *   multiples of 8, tokens less than 2^22 elements apart.  P or T may be 0 (their operands NULL).
- *   work: otpu_attn_work_bytes(...) bytes, 256-byte aligned, free again when the call's kernels ended. */
+ *   work: otpu_attn_work_bytes(...) bytes, 256-byte aligned, free again when the call's kernels ended.
+ *   The arguments come as a struct on the host, read before the call returns. */
+typedef struct otpu_attn_args {
+    int64_t bytes;                                    /* sizeof(otpu_attn_args) */
+    const void* q; int64_t qb, qt, qh;
+    const void* pk; int64_t pks, pkh;
+    const void* pv; int64_t pvs, pvh;
+    const void* k; int64_t kb, kt, kh;
+    const void* v; int64_t vb, vt, vh;
+    const int32_t* lens;
+    void* out; int64_t ob, ot, oh;
+    float* weights;
+    void* work; int64_t work_bytes;
+    int32_t B, Lq, Hq, Hkv, D, P, T, dtype;
+    double scale;
+} otpu_attn_args;
 int64_t otpu_attn_work_bytes(int B, int Lq, int Hq, int Hkv, int D, int P, int T);
-int otpu_attn_shared(const void* q, int64_t qb, int64_t qt, int64_t qh, const void* pk, int64_t pks,
-                     int64_t pkh, const void* pv, int64_t pvs, int64_t pvh, int P, const void* k, int64_t kb,
-                     int64_t kt, int64_t kh, const void* v, int64_t vb, int64_t vt, int64_t vh,
-                     const int32_t* lens, int T, int B, int Lq, int Hq, int Hkv, int D, int dtype, float scale,
-                     void* out, int64_t ob, int64_t ot, int64_t oh, float* weights, void* work,
-                     int64_t work_bytes, otpu_stream_t stream);
+int otpu_attn_shared(const otpu_attn_args* args, otpu_stream_t stream);
 
 /* Eviction from a cache by accumulated attention weight: where lens[b] > budget, each head keeps `budget`
  * slots: those whose position is among the newest `recent` (pos > max pos - recent), then by weight, the
@@ -421,11 +431,17 @@ int otpu_attn_shared(const void* q, int64_t qb, int64_t qt, int64_t qh, const vo
  *   k, v [B, T, H] rows of row_bytes bytes (a multiple of 16; strides kb, kt, kh, vb, vt, vh in bytes,
  *   multiples of 16); weights fp32 and pos int32 [B, H, T]; weights_out, pos_out and lens_out are the old
  *   arrays or ones that overlap nothing.  work: otpu_kv_evict_work_bytes(...) bytes, 256-byte aligned. */
+typedef struct otpu_evict_args {
+    int64_t bytes;                                    /* sizeof(otpu_evict_args) */
+    void* k; int64_t kb, kt, kh;
+    void* v; int64_t vb, vt, vh;
+    const float* weights; const int32_t* pos; const int32_t* lens;
+    float* weights_out; int32_t* pos_out; int32_t* lens_out;
+    void* work; int64_t work_bytes;
+    int32_t B, T, H, row_bytes, budget, recent;
+} otpu_evict_args;
 int64_t otpu_kv_evict_work_bytes(int B, int T, int H, int budget);
-int otpu_kv_evict(void* k, int64_t kb, int64_t kt, int64_t kh, void* v, int64_t vb, int64_t vt, int64_t vh,
-                  int row_bytes, const float* weights, const int32_t* pos, const int32_t* lens, int B, int T,
-                  int H, int budget, int recent, float* weights_out, int32_t* pos_out, int32_t* lens_out,
-                  void* work, int64_t work_bytes, otpu_stream_t stream);
+int otpu_kv_evict(const otpu_evict_args* args, otpu_stream_t stream);
 
 #ifdef __cplusplus
 }

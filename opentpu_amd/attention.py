@@ -76,36 +76,45 @@ def shared(q, prefix_k, prefix_v, k, v, lens, *, scale: float | None = None, wei
     if prefix_k is None and k is None:
         raise ValueError("shared: neither a prefix nor a cache")
     T = X.torch()
-    P = N = 0
-    pk = pv = kp = vp = lp = wp = None
+    P = N = pk = pv = kp = vp = lp = wp = 0
     ps = pvs = ks = vs = (0, 0, 0)
-    qs = _rows("shared", "q", q, dt, (B, Lq, Hq, D), dev)
-    if k is not None:
+    qs = q.stride()
+    if qs[3] != 1:
+        _rows("shared", "q", q, dt, (B, Lq, Hq, D), dev)
+    if k is not None:                                      # (tests in line: the functions say what is wrong)
         N, Hkv = k.shape[1], k.shape[-2]
-        ks = _rows("shared", "k", k, dt, (B, N, Hkv, D), dev)
-        vs = _rows("shared", "v", v, dt, (B, N, Hkv, D), dev)
+        own, ks, vs = (B, N, Hkv, D), k.stride(), v.stride()
+        if k.dtype != dt or k.shape != own or k.get_device() != dev or ks[3] != 1:
+            _rows("shared", "k", k, dt, own, dev)
+        if v.dtype != dt or v.shape != own or v.get_device() != dev or vs[3] != 1:
+            _rows("shared", "v", v, dt, own, dev)
         lp = _dense("shared", "lens", lens, T.int32, (B,), dev)
         kp, vp = k.data_ptr(), v.data_ptr()
     else:
         Hkv = prefix_k.shape[-2]
     if prefix_k is not None:
-        P = prefix_k.shape[0]
-        ps = _rows("shared", "prefix_k", prefix_k, dt, (P, Hkv, D), dev)
-        pvs = _rows("shared", "prefix_v", prefix_v, dt, (P, Hkv, D), dev)
+        P, ps, pvs = prefix_k.shape[0], prefix_k.stride(), prefix_v.stride()
+        pre = (P, Hkv, D)
+        if prefix_k.dtype != dt or prefix_k.shape != pre or prefix_k.get_device() != dev or ps[2] != 1:
+            _rows("shared", "prefix_k", prefix_k, dt, pre, dev)
+        if prefix_v.dtype != dt or prefix_v.shape != pre or prefix_v.get_device() != dev or pvs[2] != 1:
+            _rows("shared", "prefix_v", prefix_v, dt, pre, dev)
         pk, pv = prefix_k.data_ptr(), prefix_v.data_ptr()
     if weights is not None:
         wp = _dense("shared", "weights", weights, T.float32, (B, Hkv, N), dev)
     if out is None:
         out = T.empty_like(q, memory_format=T.contiguous_format)
-    os = _rows("shared", "out", out, dt, (B, Lq, Hq, D), dev, True)
+        os = out.stride()
+    else:
+        os = _rows("shared", "out", out, dt, (B, Lq, Hq, D), dev, True)
     if out.numel() == 0:
         return out
     nbytes = _attn_bytes(B, Lq, Hq, Hkv, D, P, N)
     work = q.new_empty((nbytes // 2 + 1,))                 # (of q's type: the least work for the host)
-    X.call("otpu_attn_shared", q.data_ptr(), qs[0], qs[1], qs[2], pk, ps[0], ps[1], pv, pvs[0], pvs[1], P, kp, ks[0],
-           ks[1], ks[2], vp, vs[0], vs[1], vs[2], lp, N, B, Lq, Hq, Hkv, D, kinds[dt],
-           D ** -0.5 if scale is None else scale, out.data_ptr(), os[0], os[1], os[2], wp, work.data_ptr(), nbytes,
-           X.stream())
+    X.call("otpu_attn_shared", X.ATTN_ARGS.pack(
+        X.ATTN_ARGS.size, q.data_ptr(), qs[0], qs[1], qs[2], pk, ps[0], ps[1], pv, pvs[0], pvs[1], kp, ks[0], ks[1], ks[2], vp,
+        vs[0], vs[1], vs[2], lp, out.data_ptr(), os[0], os[1], os[2], wp, work.data_ptr(), nbytes, B, Lq, Hq, Hkv, D, P, N,
+        kinds[dt], D ** -0.5 if scale is None else scale), X.stream())
     return out
 
 
@@ -134,8 +143,9 @@ def evict(k, v, weights, pos, lens, budget: int, recent: int = 0, *, out=None):
            _dense("evict", "out[2]", out[2], T.int32, (B,), dev))
     nbytes = _evict_bytes(B, N, H, budget)
     work = lens.new_empty((nbytes // 4 + 1,))
-    X.call("otpu_kv_evict", k.data_ptr(), e * ks[0], e * ks[1], e * ks[2], v.data_ptr(), e * vs[0], e * vs[1], e * vs[2],
-           e * D, *old, B, N, H, budget, recent, *new, work.data_ptr(), nbytes, X.stream())
+    X.call("otpu_kv_evict", X.EVICT_ARGS.pack(
+        X.EVICT_ARGS.size, k.data_ptr(), e * ks[0], e * ks[1], e * ks[2], v.data_ptr(), e * vs[0], e * vs[1], e * vs[2], *old, *new,
+        work.data_ptr(), nbytes, B, N, H, e * D, budget, recent), X.stream())
     return out
 
 

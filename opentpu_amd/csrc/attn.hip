@@ -818,15 +818,14 @@ extern "C" int64_t otpu_attn_work_bytes(int B, int Lq, int Hq, int Hkv, int D, i
     return plan(B, Lq, Hq, Hkv, D, P, T).bytes;
 }
 
-extern "C" int otpu_attn_shared(const void* q, int64_t qb, int64_t qt, int64_t qh, const void* pk, int64_t pks,
-                                int64_t pkh, const void* pv, int64_t pvs, int64_t pvh, int P, const void* k, int64_t kb,
-                                int64_t kt, int64_t kh, const void* v, int64_t vb, int64_t vt, int64_t vh,
-                                const int32_t* lens, int T, int B, int Lq, int Hq, int Hkv, int D, int dtype, float scale,
-                                void* out, int64_t ob, int64_t ot, int64_t oh, float* weights, void* work,
-                                int64_t work_bytes, otpu_stream_t stream) {
+extern "C" int otpu_attn_shared(const otpu_attn_args* args, otpu_stream_t stream) {
+    if (!args || args->bytes != (int64_t)sizeof(otpu_attn_args))
+        return otpu_fail(OTPU_EINVAL, "attn_shared: the arguments' size is not this header's %d", (int)sizeof(otpu_attn_args));
+    const auto [bytes, q, qb, qt, qh, pk, pks, pkh, pv, pvs, pvh, k, kb, kt, kh, v, vb, vt, vh, lens, out, ob, ot, oh, weights,
+                work, work_bytes, B, Lq, Hq, Hkv, D, P, T, dtype, scale] = *args;
     if (dtype != OTPU_BF16 && dtype != OTPU_F16) return otpu_fail(OTPU_EFORMAT, "attn_shared: type %d (bf16, fp16)", dtype);
     if (const int rc = check_sizes("attn_shared", B, Lq, Hq, Hkv, D, P, T)) return rc;
-    if (!(scale > 0.f) || scale > 1e30f) return otpu_fail(OTPU_EINVAL, "attn_shared: scale %g", (double)scale);
+    if (!(scale > 0.) || scale > 1e30) return otpu_fail(OTPU_EINVAL, "attn_shared: scale %g", scale);
     if (B == 0 || Lq == 0) return OTPU_OK;
     if (!q || !out || !work || (P && (!pk || !pv)) || (T && (!k || !v || !lens)))
         return otpu_fail(OTPU_EINVAL, "attn_shared: a NULL operand");
@@ -854,7 +853,7 @@ extern "C" int otpu_attn_shared(const void* q, int64_t qb, int64_t qt, int64_t q
     a.out = (char*)out; a.ob = 2 * ob; a.ot = 2 * ot; a.oh = 2 * oh;
     a.weights = weights;
     a.P = P; a.T = T; a.B = B; a.Lq = Lq; a.Hq = Hq; a.Hkv = Hkv; a.G = Hq / Hkv; a.D = D;
-    a.scale2 = scale * 1.4426950408889634f;
+    a.scale2 = (float)(scale * 1.4426950408889634);
     a.sp = p.sp; a.ss = p.ss; a.per_p = p.per_p;
     a.np = (uint32_t)p.np; a.no = (uint32_t)p.no;
     a.rows_p = p.rows_p; a.rows_o = p.rows_o;

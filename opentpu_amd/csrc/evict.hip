@@ -301,10 +301,11 @@ extern "C" int64_t otpu_kv_evict_work_bytes(int B, int T, int H, int budget) {
     return ((4 * n + 255) & ~(int64_t)255) + 8 * n * most_moves(T, budget) + 256;
 }
 
-extern "C" int otpu_kv_evict(void* k, int64_t kb, int64_t kt, int64_t kh, void* v, int64_t vb, int64_t vt, int64_t vh,
-                             int row_bytes, const float* weights, const int32_t* pos, const int32_t* lens, int B, int T,
-                             int H, int budget, int recent, float* weights_out, int32_t* pos_out, int32_t* lens_out,
-                             void* work, int64_t work_bytes, otpu_stream_t stream) {
+extern "C" int otpu_kv_evict(const otpu_evict_args* args, otpu_stream_t stream) {
+    if (!args || args->bytes != (int64_t)sizeof(otpu_evict_args))
+        return otpu_fail(OTPU_EINVAL, "kv_evict: the arguments' size is not this header's %d", (int)sizeof(otpu_evict_args));
+    const auto [bytes, k, kb, kt, kh, v, vb, vt, vh, weights, pos, lens, weights_out, pos_out, lens_out, work, work_bytes, B, T, H,
+                row_bytes, budget, recent] = *args;
     if (B < 0 || T < 0 || H < 1 || budget < 0 || recent < 0 || (int64_t)B * H > (1 << 24))
         return otpu_fail(OTPU_EINVAL, "kv_evict: B %d, T %d, H %d, budget %d, recent %d", B, T, H, budget, recent);
     if (row_bytes < 16 || row_bytes % 16 || row_bytes > (1 << 20))

@@ -39,8 +39,10 @@ def test_norm_qact():
 def attn(q=P, qs=(2048, 2048, 128), pk=P, pks=(1024, 128), pv=P, pvs=(1024, 128), np_=100, k=P, ks=(65536, 1024, 128), v=P,
          vs=(65536, 1024, 128), lens=P, T=64, B=2, Lq=1, Hq=16, Hkv=8, D=128, dtype=1, scale=0.1, out=P,
          os=(2048, 2048, 128), weights=None, work=P, nbytes=1 << 40):
-    return code("otpu_attn_shared", q, *qs, pk, *pks, pv, *pvs, np_, k, *ks, v, *vs, lens, T, B, Lq, Hq, Hkv, D, dtype, scale,
-                out, *os, weights, work, nbytes, None)
+    z = lambda x: 0 if x is None else x  # noqa: E731
+    return code("otpu_attn_shared", X.ATTN_ARGS.pack(
+        X.ATTN_ARGS.size, z(q), *qs, z(pk), *pks, z(pv), *pvs, z(k), *ks, z(v), *vs, z(lens), z(out), *os, z(weights), z(work), nbytes,
+        B, Lq, Hq, Hkv, D, np_, T, dtype, scale), None)
 
 
 def test_attn_shared():
@@ -76,7 +78,18 @@ def test_attn_work_bytes():
 
 def evict(k=P, ks=(65536, 1024, 128), v=P, vs=(65536, 1024, 128), row=128, w=P, pos=P, lens=P, B=2, T=64, H=8, budget=9,
           recent=2, wo=P, po=P, lo=P, work=P, nbytes=1 << 40):
-    return code("otpu_kv_evict", k, *ks, v, *vs, row, w, pos, lens, B, T, H, budget, recent, wo, po, lo, work, nbytes, None)
+    z = lambda x: 0 if x is None else x  # noqa: E731
+    return code("otpu_kv_evict", X.EVICT_ARGS.pack(
+        X.EVICT_ARGS.size, z(k), *ks, z(v), *vs, z(w), z(pos), z(lens), z(wo), z(po), z(lo), z(work), nbytes, B, T, H, row, budget,
+        recent), None)
+
+
+def test_structs_of_another_size():
+    """A caller built against another header: its struct's first word differs."""
+    for name, s in (("otpu_attn_shared", X.ATTN_ARGS), ("otpu_kv_evict", X.EVICT_ARGS)):
+        assert code(name, None, None) == -1
+        for size in (0, s.size - 8, s.size + 8):
+            assert code(name, size.to_bytes(8, "little") + bytes(s.size + 8), None) == -1
 
 
 def test_kv_evict():
