@@ -135,16 +135,21 @@ def evict(k, v, weights, pos, lens, budget: int, recent: int = 0, *, out=None):
     e = k.element_size()
     ks, vs = _rows("evict", "k", k, dt, (B, N, H, D), dev, True), _rows("evict", "v", v, dt, (B, N, H, D), dev, True)
     slots = (B, H, N)
-    old = (_dense("evict", "weights", weights, T.float32, slots, dev), _dense("evict", "pos", pos, T.int32, slots, dev),
-           _dense("evict", "lens", lens, T.int32, (B,), dev))
     if out is None:
         out = (T.empty_like(weights), T.empty_like(pos), T.empty_like(lens))
-    new = (_dense("evict", "out[0]", out[0], T.float32, slots, dev), _dense("evict", "out[1]", out[1], T.int32, slots, dev),
-           _dense("evict", "out[2]", out[2], T.int32, (B,), dev))
+    f32, i32 = T.float32, T.int32
+    address = []
+    for names, (w, p, n) in ((("weights", "pos", "lens"), (weights, pos, lens)), (("out[0]", "out[1]", "out[2]"), out)):
+        if not (w.dtype == f32 and p.dtype == n.dtype == i32 and w.shape == p.shape == slots and n.shape == (B,)
+                and w.get_device() == p.get_device() == n.get_device() == dev
+                and w.is_contiguous() and p.is_contiguous() and n.is_contiguous()):
+            for name, t, d, shape in zip(names, (w, p, n), (f32, i32, i32), (slots, slots, (B,))):
+                _dense("evict", name, t, d, shape, dev)
+        address += (w.data_ptr(), p.data_ptr(), n.data_ptr())
     nbytes = _evict_bytes(B, N, H, budget)
     work = lens.new_empty((nbytes // 4 + 1,))
     X.call("otpu_kv_evict", X.EVICT_ARGS.pack(
-        X.EVICT_ARGS.size, k.data_ptr(), e * ks[0], e * ks[1], e * ks[2], v.data_ptr(), e * vs[0], e * vs[1], e * vs[2], *old, *new,
+        X.EVICT_ARGS.size, k.data_ptr(), e * ks[0], e * ks[1], e * ks[2], v.data_ptr(), e * vs[0], e * vs[1], e * vs[2], *address,
         work.data_ptr(), nbytes, B, N, H, e * D, budget, recent), X.stream())
     return out
 

@@ -202,6 +202,11 @@ def quantize_ranges(x, ranges=None, row_mode: bool = False):
     return _operand(q, Sa, da, ranges, bool(row_mode))
 
 
+def _norm_refusal(name: str, t, x) -> ValueError:
+    return ValueError(f"norm_quantize: {name} is {t.dtype} {list(t.shape)}, strides {list(t.stride())}, on {t.device}; needs "
+                      f"{x.dtype} {list(x.shape)} on {x.device}, its columns adjacent, h no broadcast tensor")
+
+
 NORM_TYPES = {}                                           # torch dtype -> the ABI's type, once torch is loaded
 
 
@@ -222,30 +227,30 @@ def norm_quantize(x, gamma, residual=None, *, eps: float = 1e-6, row_mode: bool 
     if dt not in NORM_TYPES or x.dim() != 2 or dev < 0:
         raise ValueError(f"norm_quantize: x is {dt} {list(x.shape)} on {x.device}, needs [M, K] in float32, bfloat16 or float16")
     M, K = shape = x.shape
-
-    def row(name, t):
-        s = t.stride()
-        if t is not x and (t.dtype != dt or t.shape != shape or t.get_device() != dev) or (s[1] != 1 and K > 1):
-            raise ValueError(f"norm_quantize: {name} is {t.dtype} {list(t.shape)} on {t.device}, needs {dt} {[M, K]} on "
-                             f"cuda:{dev}, columns adjacent")
-        return t.data_ptr(), s[0]
-
+    xs, rp, rs, hp, hs = x.stride(), None, 0, None, 0
+    if xs[1] != 1 and K > 1:
+        raise ValueError("norm_quantize: the columns of x must be adjacent")
     if not (isinstance(gamma, T.Tensor) and gamma.dtype == T.float32 and gamma.is_contiguous() and gamma.get_device() == dev):
         gamma = X.dev(gamma, np.float32)
     if gamma.shape != (K,):
         raise ValueError(f"norm_quantize: gamma {list(gamma.shape)} over {K} columns")
-    if h is None and residual is not None:
-        h = T.empty_like(x, memory_format=T.contiguous_format)
-    if h is not None and M > 1 and h.stride(0) == 0:
-        raise ValueError("norm_quantize: h is a broadcast tensor, it cannot be written to")
-    xp, rp, hp = row("x", x), (None, 0) if residual is None else row("residual", residual), (None, 0) if h is None else row("h", h)
+    if residual is not None:
+        rp, (rs, c) = residual.data_ptr(), residual.stride() if residual.dim() == 2 else (0, 0)
+        if residual.dtype != dt or residual.shape != shape or residual.get_device() != dev or (c != 1 and K > 1):
+            raise _norm_refusal("residual", residual, x)
+        if h is None:
+            h = T.empty_like(x, memory_format=T.contiguous_format)
+    if h is not None:
+        hp, (hs, c) = h.data_ptr(), h.stride() if h.dim() == 2 else (0, 0)
+        if h.dtype != dt or h.shape != shape or h.get_device() != dev or (c != 1 and K > 1) or (hs == 0 and M > 1):
+            raise _norm_refusal("h", h, x)
     if r is not None and (r.dtype != T.float32 or r.shape != (M,) or not r.is_contiguous() or r.get_device() != dev):
         raise ValueError("norm_quantize: r is a contiguous float32 tensor [M]")
     q = T.empty_like(x, dtype=T.int8, memory_format=T.contiguous_format)
     S = gamma.new_empty((1, M))
     d = q.new_empty((M, K // 32), dtype=T.uint8)
-    X.call("otpu_norm_qact", *xp, *rp, NORM_TYPES[dt], M, K, gamma.data_ptr(), eps, X.Q_ROW if row_mode else 0, *hp,
-           None if r is None else r.data_ptr(), q.data_ptr(), K, S.data_ptr(), d.data_ptr(), K // 32, X.stream())
+    X.call("otpu_norm_qact", x.data_ptr(), xs[0], rp, rs, NORM_TYPES[dt], M, K, gamma.data_ptr(), eps,
+           X.Q_ROW if row_mode else 0, hp, hs, None if r is None else r.data_ptr(), q.data_ptr(), K, S.data_ptr(), d.data_ptr(), K // 32, X.stream())
     return _operand(q, S, d, [K], bool(row_mode)), x if h is None else h
 
 
