@@ -180,11 +180,11 @@ __device__ __forceinline__ void scores(v16f (&s)[TT], const char* ks, const v8s 
     }
 }
 
-// The running softmax over the scores of the segment's keys from `at` on: m, l and o brought up to date,
-// the weights rounded to 16 bits for the product.  lim: the segment's keys that this lane's row sees;
-// first: the least of the wave's.
-template <class E, int DP, int TT>
-__device__ __forceinline__ void softmax(Acc<DP>& a, v16f (&s)[TT], v8s (&p)[2 * TT], int at, int lim, int first, float c2) {
+// The running softmax over the scores of the segment's keys from `at` on, in two parts.  raise: scores that
+// the row does not see made -inf, m, l and o brought up to the scores' maximum.  lim: the segment's keys that
+// this lane's row sees; first: the least of the wave's.
+template <int DP, int TT>
+__device__ __forceinline__ void raise(Acc<DP>& a, v16f (&s)[TT], int at, int lim, int first, float c2) {
     const int hh = (threadIdx.x >> 5) & 1;
     if (at + 32 * TT > first) {                            // (uniform) keys that a row does not see
 #pragma unroll
@@ -211,6 +211,11 @@ __device__ __forceinline__ void softmax(Acc<DP>& a, v16f (&s)[TT], v8s (&p)[2 * 
 #pragma unroll
             for (int r = 0; r < 16; ++r) a.o[t][r] *= al;
     }
+}
+
+// The weights, their sum into l, rounded to 16 bits for the product.
+template <class E, int DP, int TT>
+__device__ __forceinline__ void weigh(Acc<DP>& a, const v16f (&s)[TT], v8s (&p)[2 * TT], float c2) {
     const float mu = a.m > -__builtin_inff() ? a.m : 0.f;  // (a row that has seen no key yet)
 #pragma unroll
     for (int t = 0; t < TT; ++t)
@@ -336,7 +341,7 @@ __device__ __forceinline__ void clear_lds(char* lds, int bytes) {
 template <class E, int DP, bool FULL, bool OWN>
 __device__ __forceinline__ void rows_part(const AttnArgs& a, char* lds, const Part& p) {
     using S = Shape<DP>;
-    constexpr int KT = S::KT, CR = S::CR;
+    constexpr int KT = S::KT, CR = S::CR, LOADS = KT / (64 / CR) / NW;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Acc<DP> c;
     c.clear();
@@ -345,27 +350,40 @@ __device__ __forceinline__ void rows_part(const AttnArgs& a, char* lds, const Pa
     load_query<DP, FULL>(qf, p.q, a.D);
     const uint32_t lds0 = lds_addr(lds);
     const int n = p.key1 - p.key0, steps = (n + KT - 1) / KT;
-    auto issue = [&](int i) INL {
-        const uint32_t to = lds0 + (uint32_t)((i & 1) * 2 * S::RB);
-        load_rows<CR, FULL, false, KT, NW>(p.k, p.ks, p.key0 + i * KT, n - 1 - i * KT, to, wave, a.D);
-        load_rows<CR, FULL, true, KT, NW>(p.v, p.vs, p.key0 + i * KT, n - 1 - i * KT, to + S::RB, wave, a.D);
+    auto keys = [&](int i) INL {
+        load_rows<CR, FULL, false, KT, NW>(p.k, p.ks, p.key0 + i * KT, n - 1 - i * KT, lds0 + (uint32_t)((i & 1) * S::RB), wave, a.D);
     };
-    issue(0);
+    auto vals = [&](int i) INL {
+        load_rows<CR, FULL, true, KT, NW>(p.v, p.vs, p.key0 + i * KT, n - 1 - i * KT, lds0 + (uint32_t)((2 + (i & 1)) * S::RB), wave, a.D);
+    };
+    keys(0);
+    vals(0);
+    if (steps > 1) keys(1);
     const int first = wave_min(p.lim), none = -wave_min(-p.lim);
     bool bad = false;
+    if (steps > 1) wait_dma<2 * LOADS>();                  // the first keys
+    else wait_dma<LOADS>();
+    bar();
+    v16f s[KT / 32], next[KT / 32];
+    v8s w[KT / 16];
+    scores<E, DP>(s, lds, qf);
+#pragma unroll 2
     for (int i = 0; i < steps; ++i) {
-        wait_dma<0>();
+        wait_dma<0>();                                     // its values, the next keys
         bar();
-        if (i + 1 < steps) issue(i + 1);
-        char* const ks = lds + (i & 1) * 2 * S::RB;
+        if (i + 1 < steps) vals(i + 1);
+        if (i + 2 < steps) keys(i + 2);
+        char* const vs = lds + (2 + (i & 1)) * S::RB;
         const int at = p.key0 + i * KT;
         if (OWN && at >= none) continue;                   // (uniform over the wave) no row of it sees these keys
-        v16f s[KT / 32];
-        v8s w[KT / 16];
-        scores<E, DP>(s, ks, qf);
-        softmax<E>(c, s, w, at, p.lim, first, a.scale2);
-        if (OWN && at + KT > p.least) bad |= finite_values<E>(ks + S::RB, KT * CR);
-        product<E, DP, KT / 32>(c, ks + S::RB, w);
+        raise(c, s, at, p.lim, first, a.scale2);
+        if (OWN && at + KT > p.least) bad |= finite_values<E>(vs, KT * CR);
+        // the next scores' products among the weights' arithmetic (after the last step of a place's old keys, unused)
+        scores<E, DP>(next, lds + ((i + 1) & 1) * S::RB, qf);
+        weigh<E>(c, s, w, a.scale2);
+        product<E, DP, KT / 32>(c, vs, w);
+#pragma unroll
+        for (int t = 0; t < KT / 32; ++t) s[t] = next[t];
     }
     store_part<DP, FULL>(a, c, swap32_sum(c.l), p);
     if constexpr (OWN)
@@ -406,7 +424,8 @@ __device__ __forceinline__ void keys_part(const AttnArgs& a, char* lds, const Pa
                 *reinterpret_cast<v4f*>(p.sc + at + 8 * r + 4 * (lane >> 5)) =
                     v4f{s[0][4 * r], s[0][4 * r + 1], s[0][4 * r + 2], s[0][4 * r + 3]};
         }
-        softmax<E>(c, s, w, at, p.lim, first, a.scale2);
+        raise(c, s, at, p.lim, first, a.scale2);
+        weigh<E>(c, s, w, a.scale2);
         if (more) wait_dma<LOADS>();                       // (the next keys' loads are younger)
         else wait_dma<0>();
         if (OWN && at + 32 > p.least) bad |= finite_values<E>(vs, 32 * CR);
