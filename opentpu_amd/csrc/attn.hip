@@ -7,6 +7,11 @@
 //   combine_kernel   the partials of a row joined and rounded to the output's type; the own tokens'
 //                    weights from their scores
 //   weights_kernel   the weights where many rows would make the scores large: from the keys again
+//
+// What bounds it, by sizes (bf16, 16 heads on 8, heads of 128): own keys and a prefix under few rows by
+// memory (64 sequences on 1024 own tokens each 5.8 TB/s, 16 rows on 65536 shared tokens 5.3); many rows by
+// the matrix units at the clock that their power leaves (8 x 512 queries on 8192 tokens 930-990 TFLOP/s; a
+// library product of 8192^3 reaches 1177); the smallest calls by launches (two, 7 us).
 #include "otpu_common.h"
 
 namespace otpu {
@@ -27,7 +32,7 @@ struct BF16 {
     static __device__ __forceinline__ v16f mma(v8s a, v8s b, v16f c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
     }
-    static constexpr uint16_t INF = 0x7F80, ONE = 0x3F80;
+    static constexpr uint16_t INF = 0x7F80;
 };
 struct F16 {
     typedef _Float16 v8 __attribute__((ext_vector_type(8)));
@@ -36,7 +41,7 @@ struct F16 {
     static __device__ __forceinline__ v16f mma(v8s a, v8s b, v16f c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
     }
-    static constexpr uint16_t INF = 0x7C00, ONE = 0x3C00;
+    static constexpr uint16_t INF = 0x7C00;
 };
 
 struct AttnArgs {
@@ -84,7 +89,8 @@ __device__ __forceinline__ float swap32_sum(float v) {
 }
 
 // Two shapes of a workgroup of four waves:
-//   rows   128 rows, 32 a wave, against the same keys: KT keys and values a step through LDS, two stages
+//   rows   128 rows, 32 a wave, against the same keys: KT keys and values a step through LDS, two places each;
+//          a step's scores are multiplied among the arithmetic of the step before
 //   keys   32 rows (or fewer) against keys that every wave takes 32 at a time for itself, without a barrier:
 //          its keys' next load is under way during the softmax and its values' product, its values' during
 //          the next scores
@@ -107,8 +113,8 @@ template <int DP_> struct Shape {
 template <int CR> __device__ __forceinline__ int kswz(int r) { return CR < 16 ? (r >> 1) & 7 : r & 15; }
 template <int CR> __device__ __forceinline__ int vswz(int r) { return CR < 16 ? 4 * ((r >> 1) & 1) : 4 * (r & 3); }
 
-// Direct loads of `rows` rows of a segment from row r0 on into LDS at `to`, dealt to nw waves of which
-// this is number w; rows past `last` read it instead.
+// Direct loads of ROWS rows of a segment from row r0 on into LDS at `to`, dealt to W waves of which this is
+// number w; rows past `last` (counted from r0) read it instead.
 template <int CR, bool FULL, bool VAL, int ROWS, int W>
 __device__ __forceinline__ void load_rows(const char* base, int64_t stride, int64_t r0, int last, uint32_t to, int w, int D) {
     constexpr int RPL = 64 / CR, LOADS = ROWS / RPL / W;   // rows a load covers, loads a wave issues
@@ -338,6 +344,9 @@ __device__ __forceinline__ void clear_lds(char* lds, int bytes) {
     bar();
 }
 
+// Two workgroups a CU, a wave of each on a SIMD: the one's products fill the other's arithmetic in part (MFMA
+// busy 54% of the cycles at 1.9 GHz).  Two groups of waves that alternate at barriers instead, products beside
+// softmax: 780 TFLOP/s against 990.  Keys loaded two steps ahead: no change, the loads are not waited for.
 template <class E, int DP, bool FULL, bool OWN>
 __device__ __forceinline__ void rows_part(const AttnArgs& a, char* lds, const Part& p) {
     using S = Shape<DP>;
@@ -390,6 +399,8 @@ __device__ __forceinline__ void rows_part(const AttnArgs& a, char* lds, const Pa
         if (any_wave(lds, bad)) add_infinite<E, KT>(a, p);
 }
 
+// No barrier until the join: a wave's loads are its own, and 64 KB of LDS a workgroup leave two on a CU, 128 KB
+// of keys and values under way or in use.
 template <class E, int DP, bool FULL, bool OWN>
 __device__ __forceinline__ void keys_part(const AttnArgs& a, char* lds, const Part& p) {
     using S = Shape<DP>;
@@ -679,8 +690,9 @@ __global__ __launch_bounds__(256) void combine_kernel(AttnArgs a, int nw) {
     if (a.lse && d == 0) a.lse[row] = m + __builtin_log2f(l);
 }
 
-// Own key weights: a wave takes 32 keys of a (sequence, head) and the R rows in tiles of 32, Q K^T with
-// the keys along the columns, so that a lane sums its key's column in registers and nothing is atomic.
+// Own key weights where R > 32 rows' scores would take more than half of the keys' bytes: a wave takes 32 keys
+// of a (sequence, head) and the R rows in tiles of 32, Q K^T with the keys along the columns, so that a lane
+// sums its key's column in registers and nothing is atomic.
 template <class E, int DP, bool FULL>
 __global__ __launch_bounds__(256) void weights_kernel(AttnArgs a) {
     constexpr int KS = DP / 16;
@@ -827,8 +839,10 @@ static int check_sizes(const char* who, int B, int Lq, int Hq, int Hkv, int D, i
     if (B < 0 || Lq < 0 || P < 0 || T < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv)
         return otpu_fail(OTPU_EINVAL, "%s: B %d, Lq %d, %d heads on %d, P %d, T %d", who, B, Lq, Hq, Hkv, P, T);
     if (D < 8 || D > 256 || D % 8) return otpu_fail(OTPU_EINVAL, "%s: heads of %d (a multiple of 8, at most 256)", who, D);
-    if ((int64_t)B * Lq * Hq > (1 << 30) || (int64_t)B * Lq * Hq * D > (1ll << 36))
-        return otpu_fail(OTPU_EINVAL, "%s: %lld rows of %d", who, (long long)B * Lq * Hq, D);
+    // (a launch holds fewer than 2^32 threads)
+    const int64_t rows = (int64_t)B * Lq * Hq;
+    if (rows > (1 << 23) || (int64_t)B * Hkv * ((T + 127) / 128) >= (1 << 24))
+        return otpu_fail(OTPU_EINVAL, "%s: %lld rows, %d sequences of %d tokens", who, (long long)rows, B, T);
     return OTPU_OK;
 }
 

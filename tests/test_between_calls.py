@@ -26,7 +26,7 @@ def test_norm_qact():
     for dtype in (0, 1, 2):
         assert norm(dtype=dtype) == 0 and norm(dtype=dtype, flags=1, d=None) == 0 and norm(dtype=dtype, res=None, h=None) == 0
     assert norm(K=32768, ldx=32768, ldr=32768, ldh=32768, ldq=32768, ldd=1024) == 0 and norm(M=0, x=None) == 0
-    for bad in (dict(K=0), dict(K=240), dict(K=32800), dict(M=-1), dict(eps=-1.0), dict(eps=float("nan")), dict(flags=2),
+    for bad in (dict(K=0), dict(K=240), dict(K=32800), dict(M=-1), dict(M=1 << 22), dict(eps=-1.0), dict(eps=float("nan")), dict(flags=2),
                 dict(x=None), dict(gamma=None), dict(q=None), dict(S=None), dict(d=None), dict(ldx=252), dict(ldr=252),
                 dict(ldh=252), dict(ldq=252), dict(ldd=7)):
         assert norm(**bad) == -1, bad
@@ -54,7 +54,7 @@ def test_attn_shared():
     for bad in (dict(Hq=15), dict(Hkv=0), dict(B=-1), dict(Lq=-1), dict(np_=-1), dict(T=-1), dict(D=4), dict(D=264), dict(D=60),
                 dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None),
                 dict(out=None), dict(work=None), dict(pk=None), dict(pv=None), dict(k=None), dict(v=None), dict(lens=None),
-                dict(nbytes=1000), dict(pks=(1 << 22, 128)), dict(ks=(65536, -1024, 128)), dict(B=1 << 20, Lq=1 << 10)):
+                dict(nbytes=1000), dict(pks=(1 << 22, 128)), dict(ks=(65536, -1024, 128)), dict(B=1 << 20, Lq=1 << 10), dict(B=1 << 18, T=1 << 20)):
         assert attn(**bad) == -1, bad
     assert attn(dtype=0) == -3 and attn(dtype=3) == -3
     for bad in (dict(q=P + 8), dict(out=P + 2), dict(pk=P + 8), dict(pv=P + 8), dict(k=P + 8), dict(v=P + 8), dict(lens=P + 2),
@@ -93,6 +93,7 @@ def test_structs_of_another_size():
 
 
 def test_kv_evict():
+    assert evict(B=1 << 19) == -1 and evict(B=(1 << 19) - 1) == 0
     assert evict() == 0 and evict(budget=64) == 0 and evict(budget=0) == 0 and evict(B=0, lens=None) == 0 and evict(row=16) == 0
     assert evict(T=0, k=None, v=None, w=None, pos=None, wo=None, po=None) == 0
     for bad in (dict(B=-1), dict(T=-1), dict(H=0), dict(budget=-1), dict(recent=-1), dict(row=8), dict(row=24), dict(row=1 << 21),

@@ -124,6 +124,17 @@ def test_some_in_place(T):
             assert np.array_equal(g.cpu().numpy(), x), which
 
 
+def test_no_slots(T):
+    """Caches without a slot: the lengths alone, in place and not."""
+    from opentpu_amd import attention
+    k = T.empty((2, 0, 3, 16), dtype=T.bfloat16, device="cuda")
+    w, pos = T.empty((2, 3, 0), device="cuda"), T.empty((2, 3, 0), dtype=T.int32, device="cuda")
+    lens = T.tensor([4, -1], dtype=T.int32, device="cuda")
+    assert attention.evict(k, k.clone(), w, pos, lens, 5)[2].tolist() == [0, 0]
+    attention.evict(k, k.clone(), w, pos, lens, 5, out=(w, pos, lens))
+    assert lens.tolist() == [0, 0]
+
+
 def test_graph(T):
     """Captured, and replayed on caches filled anew, eager work between."""
     from opentpu_amd import attention
