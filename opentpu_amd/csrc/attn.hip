@@ -272,11 +272,12 @@ struct Part {
     float* sc;                               // its scores' row, or NULL
 };
 
+// a row (of q, or of k in its place): its columns 16 s + 8 hh + 0..7, an operand of the products
 template <int DP, bool FULL>
 __device__ __forceinline__ void load_query(v8s (&qf)[DP / 16], const char* q, int D) {
     const int hh = (threadIdx.x >> 5) & 1;
 #pragma unroll
-    for (int s = 0; s < DP / 16; ++s) {                    // B operand of K Q^T
+    for (int s = 0; s < DP / 16; ++s) {
         const int c = 2 * s + hh;
         if (FULL || c * 8 < D) qf[s] = *reinterpret_cast<const v8s*>(q + c * 16);
         else qf[s] = v8s{0, 0, 0, 0, 0, 0, 0, 0};
@@ -690,56 +691,64 @@ __global__ __launch_bounds__(256) void combine_kernel(AttnArgs a, int nw) {
     if (a.lse && d == 0) a.lse[row] = m + __builtin_log2f(l);
 }
 
-// Own key weights where R > 32 rows' scores would take more than half of the keys' bytes: a wave takes 32 keys
-// of a (sequence, head) and the R rows in tiles of 32, Q K^T with the keys along the columns, so that a lane
-// sums its key's column in registers and nothing is atomic.
+// Own key weights where R > 32 rows' scores would take more than half of the keys' bytes: a workgroup takes 32
+// keys of a (sequence, head), its waves the rows in tiles of 32 by turns.  As in `scores` a lane has one row
+// and 16 of the keys, so that the row's lse is its own and the sums over row tiles stay in registers; lanes and
+// waves are summed once at the end, in one order, and nothing is atomic.  (82 x 13 queries for 5 heads on 786
+// own tokens 32 us; 128 keys a workgroup, so that the queries are read less often, 39: fewer waves a SIMD.)
 template <class E, int DP, bool FULL>
-__global__ __launch_bounds__(256) void weights_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64) void weights_kernel(AttnArgs a) {
     constexpr int KS = DP / 16;
+    __shared__ float part[NW][32];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r32 = lane & 31, hh = lane >> 5;
     const int R = a.Lq * a.G;
     const int h = blockIdx.x % a.Hkv;
-    int x = blockIdx.x / a.Hkv;
-    const int nt = (a.T + 127) / 128;
-    const int b = x / nt, t0 = (x % nt) * 128 + wave * 32;
-    const int len = min(max(a.lens[b], 0), a.T);
-    if (t0 >= len) return;
-    const int key = t0 + r32;
-    const char* const krow = a.k + b * a.kb + h * a.kh + (int64_t)min(key, len - 1) * a.kt;
+    const int x = blockIdx.x / a.Hkv;
+    const int nt = (a.T + 31) / 32;
+    const int b = x / nt, t0 = (x % nt) * 32;
+    const int len = min(max(a.lens[b], 0), a.T), own = len - a.Lq;
+    if (t0 >= len) return;                                 // (uniform over the workgroup)
+    const char* const krow = a.k + b * a.kb + h * a.kh + (int64_t)min(t0 + r32, len - 1) * a.kt;
     v8s kf[KS];
+    load_query<DP, FULL>(kf, krow, a.D);
+    float sum[16];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-        const int c = 2 * s + hh;
-        if (FULL || c * 8 < a.D) kf[s] = *reinterpret_cast<const v8s*>(krow + c * 16);
-        else kf[s] = v8s{0, 0, 0, 0, 0, 0, 0, 0};
-    }
-    float sum = 0.f;
-    for (int m0 = 0; m0 < R; m0 += 32) {
-        const int mc = min(m0 + r32, R - 1), i = mc / a.G, g = mc - i * a.G;
-        const char* const qrow = a.q + b * a.qb + i * a.qt + (h * a.G + g) * a.qh;
+    for (int r = 0; r < 16; ++r) sum[r] = 0.f;
+    // rows of tokens before own + t0 see none of the keys
+    for (int m0 = (max(t0 - own, 0) * a.G & ~31) + 32 * wave; m0 < R; m0 += 32 * NW) {
+        const int mc = min(m0 + r32, R - 1), i = mc / a.G, head = h * a.G + mc - i * a.G;
+        const float lse = a.lse[((int64_t)b * a.Lq + i) * a.Hq + head];
+        v8s qf[KS];
+        load_query<DP, FULL>(qf, a.q + b * a.qb + i * a.qt + head * a.qh, a.D);
         v16f s;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
-        for (int u = 0; u < KS; ++u) {
-            const int c = 2 * u + hh;
-            v8s qf = v8s{0, 0, 0, 0, 0, 0, 0, 0};
-            if (FULL || c * 8 < a.D) qf = *reinterpret_cast<const v8s*>(qrow + c * 16);
-            s = E::mma(qf, kf[u], s);
-        }
+        for (int u = 0; u < KS; ++u) s = E::mma(kf[u], qf[u], s);
+        const int see = m0 + r32 < R ? own + i : -1;       // the row's own token
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int mr = m0 + 8 * (r / 4) + 4 * hh + r % 4;
-            if (mr < R) {
-                const int ii = mr / a.G, gg = mr - ii * a.G;
-                if (key <= len - a.Lq + ii)
-                    sum += __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.scale2, -a.lse[((int64_t)b * a.Lq + ii) * a.Hq + h * a.G + gg]));
-            }
-        }
+        for (int r = 0; r < 16; ++r)
+            if (t0 + 8 * (r / 4) + 4 * hh + r % 4 <= see) sum[r] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.scale2, -lse));
     }
-    sum = swap32_sum(sum);
-    if (hh == 0 && key < len) a.weights[((int64_t)b * a.Hkv + h) * a.T + key] += sum;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        float v = sum[r];                                  // over the 32 rows: DPP within 16 lanes, then their pair
+        v += bitsf((uint32_t)__builtin_amdgcn_update_dpp(0, (int)fbits(v), 0xB1, 0xF, 0xF, false));
+        v += bitsf((uint32_t)__builtin_amdgcn_update_dpp(0, (int)fbits(v), 0x4E, 0xF, 0xF, false));
+        v += bitsf((uint32_t)__builtin_amdgcn_update_dpp(0, (int)fbits(v), 0x141, 0xF, 0xF, false));
+        v += bitsf((uint32_t)__builtin_amdgcn_update_dpp(0, (int)fbits(v), 0x140, 0xF, 0xF, false));
+        const auto p = __builtin_amdgcn_permlane16_swap(fbits(v), fbits(v), false, false);
+        v = bitsf(p[0]) + bitsf(p[1]);
+        if (r32 == 0) part[wave][8 * (r / 4) + 4 * hh + r % 4] = v;
+    }
+    __syncthreads();
+    if (threadIdx.x < 32 && t0 + (int)threadIdx.x < len) {
+        float v = part[0][threadIdx.x];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) v += part[w][threadIdx.x];
+        a.weights[((int64_t)b * a.Hkv + h) * a.T + t0 + threadIdx.x] += v;
+    }
 }
 
 // ---- the host's side --------------------------------------------------------------------------
@@ -758,9 +767,10 @@ static Plan plan(int B, int Lq, int Hq, int Hkv, int D, int P, int T) {
     const int R = Lq * (Hq / Hkv);
     const int64_t M = (int64_t)B * R, slots = 2 * (int64_t)otpu_cu_count();
     p.rows = (int64_t)B * Lq * Hq;
-    auto tile = [&](int64_t m) { return m <= 32 ? 32 : 32 * NW; };
-    p.rows_p = tile(M);
-    p.rows_o = tile(R);
+    // (own keys of up to 64 rows: two tiles of 32 read them from the L2; 16 x 24 queries for 2 heads on 200 own
+    // tokens 18.4 us, a tile of 128 21.4.  A prefix: no difference.)
+    p.rows_p = M <= 32 ? 32 : 32 * NW;
+    p.rows_o = R <= 64 ? 32 : 32 * NW;
     const int64_t gp = (int64_t)Hkv * ((M + p.rows_p - 1) / p.rows_p);
     const int64_t go = (int64_t)B * Hkv * ((R + p.rows_o - 1) / p.rows_o);
     // Splits: as many as fill the places of the CUs, of `least` keys or more.
@@ -784,7 +794,7 @@ static Plan plan(int B, int Lq, int Hq, int Hkv, int D, int P, int T) {
     p.sp = (int)s;
     p.per_p = p.sp ? ((P + p.sp - 1) / p.sp + 31) & ~31 : 0;
     p.np = gp * p.sp;
-    p.scores = p.rows_o == 32;
+    p.scores = R <= 32;
     p.tp = (T + 31) & ~31;
     const int64_t n = p.sp + p.ss;
     auto part = [&](int64_t floats) {
@@ -817,7 +827,7 @@ static void launch_all(const AttnArgs& a, const Plan& p, hipStream_t s) {
     else if (n > 2) launch_combine<E, 2>(a, p, s);
     else launch_combine<E, 1>(a, p, s);
     if (a.weights && a.T && !a.sc)
-        weights_kernel<E, DP, FULL><<<(unsigned)((int64_t)a.B * a.Hkv * ((a.T + 127) / 128)), 256, 0, s>>>(a);
+        weights_kernel<E, DP, FULL><<<(unsigned)((int64_t)a.B * a.Hkv * ((a.T + 31) / 32)), NW * 64, 0, s>>>(a);
 }
 
 template <class E>
@@ -841,7 +851,7 @@ static int check_sizes(const char* who, int B, int Lq, int Hq, int Hkv, int D, i
     if (D < 8 || D > 256 || D % 8) return otpu_fail(OTPU_EINVAL, "%s: heads of %d (a multiple of 8, at most 256)", who, D);
     // (a launch holds fewer than 2^32 threads)
     const int64_t rows = (int64_t)B * Lq * Hq;
-    if (rows > (1 << 23) || (int64_t)B * Hkv * ((T + 127) / 128) >= (1 << 24))
+    if (rows > (1 << 23) || (int64_t)B * Hkv * ((T + 31) / 32) >= (1 << 24))
         return otpu_fail(OTPU_EINVAL, "%s: %lld rows, %d sequences of %d tokens", who, (long long)rows, B, T);
     return OTPU_OK;
 }
