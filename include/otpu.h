@@ -427,7 +427,7 @@ int otpu_attn_shared(const otpu_attn_args* args, otpu_stream_t stream);
  * lower slot where weights are equal (a NaN weight counts as the largest).  The j-th slot below budget
  * that goes is overwritten by the j-th slot at or past budget that stays (rows of k and v in place, its
  * weight and position); slots keep no order.  lens_out[b] = min(lens[b], budget); slots from there on get
- * weight 0 and position -1.
+ * weight 0 and position -1.  T at most 2^30.
  *   k, v [B, T, H] rows of row_bytes bytes (a multiple of 16; strides kb, kt, kh, vb, vt, vh in bytes,
  *   multiples of 16); weights fp32 and pos int32 [B, H, T]; weights_out, pos_out and lens_out are the old
  *   arrays or ones that overlap nothing.  work: otpu_kv_evict_work_bytes(...) bytes, 256-byte aligned. */

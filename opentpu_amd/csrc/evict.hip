@@ -12,7 +12,7 @@
 // The moves are bound by memory (64 x 8 caches of 2048 slots cut to 1000: 268 MB read and written, 63 us with
 // the selection, 4.3 TB/s; a copy reaches 5.1).  The selection is a chain of a few trips to memory, three
 // passes over keys in registers with three barriers each, and a scan: 8 us for 256 caches of 1024 slots with
-// the launch, ~25 for caches of 32768, where one workgroup's instructions bound it.
+// the launch, 30 for caches of 32768, where one workgroup's instructions bound it.
 #include "otpu_common.h"
 
 namespace otpu {
@@ -310,7 +310,7 @@ extern "C" int otpu_kv_evict(const otpu_evict_args* args, otpu_stream_t stream) 
         return otpu_fail(OTPU_EINVAL, "kv_evict: the arguments' size is not this header's %d", (int)sizeof(otpu_evict_args));
     const auto [bytes, k, kb, kt, kh, v, vb, vt, vh, weights, pos, lens, weights_out, pos_out, lens_out, work, work_bytes, B, T, H,
                 row_bytes, budget, recent] = *args;
-    if (B < 0 || T < 0 || H < 1 || budget < 0 || recent < 0 || (int64_t)B * H >= (1 << 22))
+    if (B < 0 || T < 0 || T > (1 << 30) || H < 1 || budget < 0 || recent < 0 || (int64_t)B * H >= (1 << 22))
         return otpu_fail(OTPU_EINVAL, "kv_evict: B %d, T %d, H %d, budget %d, recent %d", B, T, H, budget, recent);
     if (row_bytes < 16 || row_bytes % 16 || row_bytes > (1 << 20))
         return otpu_fail(OTPU_EINVAL, "kv_evict: rows of %d bytes (a multiple of 16)", row_bytes);

@@ -96,7 +96,7 @@ def test_kv_evict():
     assert evict(B=1 << 19) == -1 and evict(B=(1 << 19) - 1) == 0
     assert evict() == 0 and evict(budget=64) == 0 and evict(budget=0) == 0 and evict(B=0, lens=None) == 0 and evict(row=16) == 0
     assert evict(T=0, k=None, v=None, w=None, pos=None, wo=None, po=None) == 0
-    for bad in (dict(B=-1), dict(T=-1), dict(H=0), dict(budget=-1), dict(recent=-1), dict(row=8), dict(row=24), dict(row=1 << 21),
+    for bad in (dict(B=-1), dict(T=-1), dict(T=(1 << 30) + 1), dict(H=0), dict(budget=-1), dict(recent=-1), dict(row=8), dict(row=24), dict(row=1 << 21),
                 dict(k=None), dict(v=None), dict(w=None), dict(pos=None), dict(lens=None), dict(wo=None), dict(po=None),
                 dict(lo=None), dict(work=None), dict(nbytes=64)):
         assert evict(**bad) == -1, bad
