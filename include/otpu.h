@@ -402,7 +402,8 @@ int otpu_norm_qact(const void* x, int64_t ldx, const void* res, int64_t ldr, int
  *   [B, Hkv, T] fp32: the own tokens' softmax weights, summed over the Lq queries and the head's Hq / Hkv
  *   query heads, are added to it.  dtype OTPU_BF16 or OTPU_F16 for q, caches and out; sums, maxima and
  *   weights fp32.  D a multiple of 8, at most 256; scale > 0; addresses 16-byte aligned, strides
- *   multiples of 8, tokens less than 2^22 elements apart.  P or T may be 0 (their operands NULL).
+ *   multiples of 8, tokens less than 2^22 elements apart.  P and T at most 2^30, either may
+ *   be 0 (its operands NULL).
  *   work: otpu_attn_work_bytes(...) bytes, 256-byte aligned, free again when the call's kernels ended.
  *   The arguments come as a struct on the host, read before the call returns. */
 typedef struct otpu_attn_args {
@@ -423,8 +424,8 @@ int64_t otpu_attn_work_bytes(int B, int Lq, int Hq, int Hkv, int D, int P, int T
 int otpu_attn_shared(const otpu_attn_args* args, otpu_stream_t stream);
 
 /* Eviction from a cache by accumulated attention weight: where lens[b] > budget, each head keeps `budget`
- * slots: those whose position is among the newest `recent` (pos > max pos - recent), then by weight, the
- * lower slot where weights are equal (a NaN weight counts as the largest).  The j-th slot below budget
+ * slots: those whose position is among the newest `recent` (pos > max pos - recent; of more than budget the
+ * lower slots), then by weight, the lower slot where weights are equal (a NaN weight counts as the largest).  The j-th slot below budget
  * that goes is overwritten by the j-th slot at or past budget that stays (rows of k and v in place, its
  * weight and position); slots keep no order.  lens_out[b] = min(lens[b], budget); slots from there on get
  * weight 0 and position -1.  T at most 2^30.

@@ -120,7 +120,7 @@ def shared(q, prefix_k, prefix_v, k, v, lens, *, scale: float | None = None, wei
 
 def evict(k, v, weights, pos, lens, budget: int, recent: int = 0, *, out=None):
     """Frees slots of the caches k, v [B, T, H, D] in place: where lens[b] > budget, each head keeps `budget`
-    slots, those of its `recent` newest positions first, then those of the largest accumulated weights, the
+    slots, those of its `recent` newest positions first (of more than `budget` the lower slots), then those of the largest accumulated weights, the
     lower slot where they are equal.  Slots below budget that go are overwritten by the slots past it
     that stay (both in slot order), so slots keep no order of positions.
 

@@ -166,6 +166,13 @@ __device__ __forceinline__ bool finite_values(char* vs, int pieces) {
     return __any(found);
 }
 
+// Places past the segment's last key hold its values again: zeros instead, as an infinity would meet their
+// weights of 0.
+template <int CR>
+__device__ __forceinline__ void clear_tail(char* vs, int from, int rows) {
+    for (int x = from * CR + (int)(threadIdx.x & 63); x < rows * CR; x += 64) reinterpret_cast<v4u*>(vs)[x] = v4u{0, 0, 0, 0};
+}
+
 // S^T = K Q^T of 32 TT keys at ks (LDS): a lane has its row's scores of keys 8 r + 4 hh + 0..3 of each 32
 template <class E, int DP, int TT>
 __device__ __forceinline__ void scores(v16f (&s)[TT], const char* ks, const v8s (&qf)[DP / 16]) {
@@ -205,10 +212,12 @@ __device__ __forceinline__ void raise(Acc<DP>& a, v16f (&s)[TT], int at, int lim
 #pragma unroll
         for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[t][r]);
     mt = swap32_max(mt) * c2;
-    // the maximum is raised, and o and l scaled, only where a score passes it by more than 2^8: the
-    // weights stay below 2^8, exact in the same relative terms
-    if (__any(mt > a.m + 8.f)) {
-        const float mn = fmaxf(a.m, mt);
+    // m is raised, and o and l scaled, only where a score passes it by more than 15, and then to 7 under the
+    // score: weights of 2^7 to 2^15 for the largest keep fp16's subnormals (an error of 2^-25 whatever the
+    // weight) 2^-32 below it, which 2^17 keys of one small weight would show otherwise; to fp32 sums and bf16
+    // any m is the same
+    if (__any(mt > a.m + 15.f)) {
+        const float mn = fmaxf(a.m, mt - 7.f);
         const float al = mn > -__builtin_inff() ? __builtin_amdgcn_exp2f(a.m - mn) : 1.f;
         a.m = mn;
         a.l *= al;
@@ -288,7 +297,8 @@ template <int DP, bool FULL>
 __device__ __forceinline__ void store_part(const AttnArgs& a, const Acc<DP>& c, float l, const Part& p) {
     if (!p.valid) return;
     const int hh = (threadIdx.x >> 5) & 1;
-    if (hh == 0) { a.pm[p.at] = c.m; a.pl[p.at] = l; }
+    // (a sum that is NaN counts in the join, also where no score was a number and raised m)
+    if (hh == 0) { a.pm[p.at] = l == l ? c.m : 0.f; a.pl[p.at] = l; }
     float* const po = a.po + p.at * a.D;
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t)
@@ -388,6 +398,7 @@ __device__ __forceinline__ void rows_part(const AttnArgs& a, char* lds, const Pa
         if (OWN && at >= none) continue;                   // (uniform over the wave) no row of it sees these keys
         raise(c, s, at, p.lim, first, a.scale2);
         if (OWN && at + KT > p.least) bad |= finite_values<E>(vs, KT * CR);
+        if (!OWN && at + KT > p.key1) clear_tail<CR>(vs, p.key1 - at, KT);
         // the next scores' products among the weights' arithmetic (after the last step of a place's old keys, unused)
         scores<E, DP>(next, lds + ((i + 1) & 1) * S::RB, qf);
         weigh<E>(c, s, w, a.scale2);
@@ -441,6 +452,7 @@ __device__ __forceinline__ void keys_part(const AttnArgs& a, char* lds, const Pa
         if (more) wait_dma<LOADS>();                       // (the next keys' loads are younger)
         else wait_dma<0>();
         if (OWN && at + 32 > p.least) bad |= finite_values<E>(vs, 32 * CR);
+        if (!OWN && at + 32 > p.key1) clear_tail<CR>(vs, p.key1 - at, 32);
         product<E, DP, 1>(c, vs, w);
         asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
         if (more) vals(j + NW);
@@ -846,7 +858,7 @@ using namespace otpu;
 static bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 static int check_sizes(const char* who, int B, int Lq, int Hq, int Hkv, int D, int P, int T) {
-    if (B < 0 || Lq < 0 || P < 0 || T < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv)
+    if (B < 0 || Lq < 0 || P < 0 || P > (1 << 30) || T < 0 || T > (1 << 30) || Hq < 1 || Hkv < 1 || Hq % Hkv)
         return otpu_fail(OTPU_EINVAL, "%s: B %d, Lq %d, %d heads on %d, P %d, T %d", who, B, Lq, Hq, Hkv, P, T);
     if (D < 8 || D > 256 || D % 8) return otpu_fail(OTPU_EINVAL, "%s: heads of %d (a multiple of 8, at most 256)", who, D);
     // (a launch holds fewer than 2^32 threads)

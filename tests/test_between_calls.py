@@ -51,7 +51,7 @@ def test_attn_shared():
             assert attn(dtype=dtype, D=D) == 0 and attn(dtype=dtype, D=D, weights=P) == 0
     assert attn(np_=0, pk=None, pv=None) == 0 and attn(T=0, k=None, v=None, lens=None) == 0
     assert attn(B=0) == 0 and attn(Lq=0) == 0 and attn(qs=(0, 0, 0)) == 0
-    for bad in (dict(Hq=15), dict(Hkv=0), dict(B=-1), dict(Lq=-1), dict(np_=-1), dict(T=-1), dict(D=4), dict(D=264), dict(D=60),
+    for bad in (dict(Hq=15), dict(Hkv=0), dict(B=-1), dict(Lq=-1), dict(np_=-1), dict(np_=(1 << 30) + 1), dict(T=-1), dict(T=(1 << 30) + 1), dict(D=4), dict(D=264), dict(D=60),
                 dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None),
                 dict(out=None), dict(work=None), dict(pk=None), dict(pv=None), dict(k=None), dict(v=None), dict(lens=None),
                 dict(nbytes=1000), dict(pks=(1 << 22, 128)), dict(ks=(65536, -1024, 128)), dict(B=1 << 20, Lq=1 << 10), dict(B=1 << 18, T=1 << 20)):

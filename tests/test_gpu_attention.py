@@ -271,3 +271,77 @@ def test_no_queries_and_refusals(T):
                 lambda: attention.shared(q[..., 4:60], pk[..., 4:60], pv[..., 4:60], k[..., 4:60], v[..., 4:60], lens)):
         with pytest.raises(X.OtpuError):
             bad()
+
+
+@pytest.mark.parametrize("dt", ["bfloat16", "float16"])
+def test_what_is_no_number_is_not_lost(T, dt):
+    """A NaN in a query makes its row and the weights it adds NaN, though it raises no maximum; a key's NaN every row
+    that sees it; no other row changes.  Few rows and many, a prefix and a cache alone and together."""
+    from opentpu_amd import attention
+    rng = np.random.default_rng(21)
+    dt = getattr(T, dt)
+    nan = float("nan")
+    for B, Lq, Hq, Hkv, D, P, Tn in ((3, 1, 4, 2, 128, 40, 9), (3, 1, 4, 2, 64, 0, 300), (2, 3, 2, 1, 96, 700, 0),
+                                     (2, 50, 6, 2, 128, 200, 60), (70, 1, 4, 1, 128, 1025, 40), (2, 9, 2, 2, 256, 90, 12)):
+        say("no number", dt, B, Lq, Hq, Hkv, D, P, Tn)
+        q, pk, pv, k, v, _ = (t.cuda() for t in make(T, rng, dt, B, Lq, Hq, Hkv, D, P, Tn))
+        lens = T.full((B,), Tn, dtype=T.int32, device="cuda")
+        w0 = T.zeros((B, Hkv, Tn), device="cuda")
+        want = attention.shared(q, pk, pv, k, v, lens, weights=w0)
+        q2, w = q.clone(), T.zeros_like(w0)
+        q2[1, Lq - 1, 1, 5] = nan
+        got = attention.shared(q2, pk, pv, k, v, lens, weights=w)
+        hit = T.zeros((B, Lq, Hq), dtype=T.bool, device="cuda")
+        hit[1, Lq - 1, 1] = True
+        assert bool(T.isnan(got[hit]).all()) and T.equal(got[~hit], want[~hit])
+        if Tn:
+            head = T.zeros((B, Hkv), dtype=T.bool, device="cuda")
+            head[1, 1 * Hkv // Hq] = True                 # (query head 1's)
+            assert bool(T.isnan(w[head]).all()) and T.equal(w[~head], w0[~head])
+        if P:
+            pk2 = pk.clone()
+            pk2[P - 1, 0, 3] = nan
+            got = attention.shared(q, pk2, pv, k, v, lens)
+            G = Hq // Hkv
+            assert bool(T.isnan(got[:, :, :G]).all()) and T.equal(got[:, :, G:], want[:, :, G:])
+
+
+@pytest.mark.parametrize("dt", ["bfloat16", "float16"])
+def test_infinities_at_the_end_of_a_prefix(T, dt):
+    """The values of a prefix's last token, which the last step's places past it repeat."""
+    from opentpu_amd import attention
+    rng = np.random.default_rng(22)
+    dt = getattr(T, dt)
+    inf = float("inf")
+    for B, Lq, Hq, Hkv, D, P in ((2, 1, 2, 1, 128, 33), (2, 1, 2, 1, 64, 500), (40, 2, 2, 1, 128, 65), (40, 2, 2, 1, 72, 1000), (3, 1, 1, 1, 256, 50),
+                                 (40, 2, 2, 1, 256, 50)):
+        say("end of a prefix", dt, B, Lq, Hq, Hkv, D, P)
+        q, pk, pv, *_ = (t.cuda() for t in make(T, rng, dt, B, Lq, Hq, Hkv, D, P, 0))
+        want = attention.shared(q, pk, pv, None, None, None)
+        pv[P - 1, :, 3], pv[P - 1, :, 4] = inf, -inf
+        got = attention.shared(q, pk, pv, None, None, None)
+        assert bool((got[..., 3] == inf).all()) and bool((got[..., 4] == -inf).all())
+        got[..., 3:5] = want[..., 3:5]
+        assert T.equal(got, want)
+
+
+def test_many_small_weights(T):
+    """One key far above 2^17 others of one score: their weights are under fp16's subnormals, their sum is not small.
+    Bound: rounding a weight 2^-11 or, within 2^-32 of the largest, 2^-25 absolute against its scale of 2^7 or more; the
+    output's rounding 2^-11; and fp32 sums of 2^17 terms in parts of at most 2^12 (a relative 2^-12 of what they add up)."""
+    from opentpu_amd import attention
+    P, D = 1 << 17, 64
+    q = T.zeros((1, 1, 1, D), dtype=T.float16, device="cuda")
+    q[..., 0] = 1.0
+    pv = T.ones((P, 1, D), dtype=T.float16, device="cuda")
+    for gap in (9.0, 13.0, 16.0, 17.0, 17.5):
+        for place in (0, 70000, P - 1):
+            pk = T.zeros((P, 1, D), dtype=T.float16, device="cuda")
+            pk[place, 0, 0] = gap
+            pv[:] = 1
+            pv[place] = 0
+            got = attention.shared(q, pk, pv, None, None, None, scale=1.0).double()
+            mass = (P - 1) * math.exp(-gap)
+            want = mass / (1 + mass)
+            bound = want * (2.0 ** -11 + 2.0 ** -11 + 2.0 ** -12) + P * 2.0 ** -32 + 2.0 ** -25
+            assert float((got - want).abs().max()) <= bound, (gap, place, float(got[0, 0, 0, 0]), want, bound)
