@@ -7,7 +7,7 @@
 //   evict_select_kernel   a workgroup a (sequence, head): the threshold by radix selection (11, 11 and 10
 //                         bits), the holes and their sources, the slots' weights and positions; up to 64
 //                         rows of k and v
-//   evict_move_kernel     more rows of k and v
+//   evict_move_kernel     more rows of k and v, and the slots that are free
 //
 // The moves are bound by memory (64 x 8 caches of 2048 slots cut to 1000: 268 MB read and written, 63 us with
 // the selection, 4.3 TB/s; a copy reaches 5.1).  The selection is a chain of a few trips to memory, three
@@ -122,7 +122,7 @@ __global__ __launch_bounds__(EW, KPT <= 2 ? 8 : 4) void evict_select_kernel(Evic
     if (tid == 0 && bh % a.H == 0 && a.ln != a.lens) a.ln[b] = left;
 
     if (n <= a.budget || a.budget == 0) {    // every slot stays, or none
-        for (int t = tid; t < a.T; t += EW) {
+        for (int t = tid; t < (a.here ? a.T : left); t += EW) {
             wn[t] = t < left ? w[t] : 0.f;
             pn[t] = t < left ? pos[t] : -1;
         }
@@ -258,8 +258,10 @@ __global__ __launch_bounds__(EW, KPT <= 2 ? 8 : 4) void evict_select_kernel(Evic
         pn[m.x] = pos[m.y];
     }
     if (a.here) move_rows<EW, 1>(a, a.k + b * a.kb + (bh - b * a.H) * a.kh, a.v + b * a.vb + (bh - b * a.H) * a.vh, mv, holes, 0, 1);
-    __syncthreads();                          // the sources are read, in place too
-    for (int t = left + tid; t < a.T; t += EW) { wn[t] = 0.f; pn[t] = -1; }
+    if (a.here) {
+        __syncthreads();                      // the sources are read, in place too
+        for (int t = left + tid; t < a.T; t += EW) { wn[t] = 0.f; pn[t] = -1; }
+    }
     if (tid == 0) a.count[bh] = holes;
 }
 
@@ -272,6 +274,13 @@ __global__ __launch_bounds__(256) void evict_lens_kernel(EvictArgs a) { store_le
 __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
     const int bh = blockIdx.x, b = bh / a.H, h = bh - b * a.H;
     if (bh == 0 && blockIdx.y == 0 && a.ln == a.lens) store_lens(a);
+    // the slots past the new length (the same from the old length and the new one).  Here and not in the
+    // selection: one workgroup's stores to most of a long cache would make everything wait
+    const int left = min(min(max(a.lens[b], 0), a.T), a.budget);
+    for (int64_t t = left + (int)(blockIdx.y * 256 + threadIdx.x); t < a.T; t += 256 * (int64_t)gridDim.y) {
+        a.wn[(int64_t)bh * a.T + t] = 0.f;
+        a.pn[(int64_t)bh * a.T + t] = -1;
+    }
     move_rows<256, 4>(a, a.k + b * a.kb + h * a.kh, a.v + b * a.vb + h * a.vh, a.moves + (int64_t)bh * a.most, a.count[bh],
                    blockIdx.y, gridDim.y);
 }
