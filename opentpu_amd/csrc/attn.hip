@@ -58,6 +58,7 @@ struct AttnArgs {
     int sp, ss, per_p;                       // splits of the prefix, of the own keys; keys of a prefix split
     uint32_t np, no;                         // workgroups of the prefix, of the own keys
     int rows_p, rows_o;                      // rows of their tiles: 32 or 128
+    bool whole;                              // one segment, D <= 128: a row's share is its output, nothing to join
     float* po;                               // partial o [sp + ss][rows][D]
     float* pm;                               // m [sp + ss][rows]
     float* pl;                               // l [sp + ss][rows]
@@ -293,10 +294,32 @@ __device__ __forceinline__ void load_query(v8s (&qf)[DP / 16], const char* q, in
     }
 }
 
-template <int DP, bool FULL>
+// the output's row of a place among the partials of the only segment
+__device__ __forceinline__ char* out_row(const AttnArgs& a, int64_t at) {
+    const int row = (int)at, bi = row / a.Hq, head = row - bi * a.Hq, b = bi / a.Lq;
+    return a.out + b * a.ob + (bi - b * a.Lq) * a.ot + head * a.oh;
+}
+
+template <class E, int DP, bool FULL>
 __device__ __forceinline__ void store_part(const AttnArgs& a, const Acc<DP>& c, float l, const Part& p) {
     if (!p.valid) return;
     const int hh = (threadIdx.x >> 5) & 1;
+    // (a join of 4096 x 16 rows takes 17 us, a launch 2.5; heads of 256 have no registers for it)
+    if (DP <= 128 && a.whole) {
+        char* const out = out_row(a, p.at);
+        const float il = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int d = t * 32 + 8 * r + 4 * hh;
+                typename E::v4 z;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) z[j] = (typename E::e)(c.o[t][4 * r + j] * il);
+                if (FULL || d < a.D) *reinterpret_cast<typename E::v4*>(out + 2 * d) = z;
+            }
+        return;
+    }
     // (a sum that is NaN counts in the join, also where no score was a number and raised m)
     if (hh == 0) { a.pm[p.at] = l == l ? c.m : 0.f; a.pl[p.at] = l; }
     float* const po = a.po + p.at * a.D;
@@ -312,7 +335,7 @@ __device__ __forceinline__ void store_part(const AttnArgs& a, const Acc<DP>& c, 
 
 // the values that finite_values took out, from keys of tiles of KT, added to the partials of the wave's rows
 // that see them
-template <class E, int KT>
+template <class E, int DP, int KT>
 __device__ __forceinline__ void add_infinite(const AttnArgs& a, const Part& p) {
     const int lane = threadIdx.x & 63;
     const int from = p.key0 + max(p.least - p.key0, 0) / KT * KT;
@@ -320,14 +343,17 @@ __device__ __forceinline__ void add_infinite(const AttnArgs& a, const Part& p) {
     for (int r = 0; r < 32; ++r) {
         if (!__shfl((int)p.valid, r, 64)) continue;
         const int lim = __shfl(p.lim, r, 64);
-        float* const po = a.po + __shfl(p.at, r, 64) * a.D;
+        const int64_t at = __shfl(p.at, r, 64);
+        float* const po = a.po + at * a.D;
+        typename E::e* const out = reinterpret_cast<typename E::e*>(out_row(a, at));
         for (int d = lane; d < a.D; d += 64) {
             float add = 0.f;
             for (int t = from; t < lim; ++t) {
                 const float x = (float)reinterpret_cast<const typename E::e*>(p.v + (int64_t)t * p.vs)[d];
                 if (!(__builtin_fabsf(x) < __builtin_inff())) add += x;
             }
-            if (add != 0.f) po[d] += add;
+            if (DP <= 128 && add != 0.f && a.whole) out[d] = (typename E::e)((float)out[d] + add);
+            else if (add != 0.f) po[d] += add;
         }
     }
 }
@@ -406,9 +432,9 @@ __device__ __forceinline__ void rows_part(const AttnArgs& a, char* lds, const Pa
 #pragma unroll
         for (int t = 0; t < KT / 32; ++t) s[t] = next[t];
     }
-    store_part<DP, FULL>(a, c, swap32_sum(c.l), p);
+    store_part<E, DP, FULL>(a, c, swap32_sum(c.l), p);
     if constexpr (OWN)
-        if (any_wave(lds, bad)) add_infinite<E, KT>(a, p);
+        if (any_wave(lds, bad)) add_infinite<E, DP, KT>(a, p);
 }
 
 // No barrier until the join: a wave's loads are its own, and 64 KB of LDS a workgroup leave two on a CU, 128 KB
@@ -487,9 +513,9 @@ __device__ __forceinline__ void keys_part(const AttnArgs& a, char* lds, const Pa
             for (int r = 0; r < 16; ++r) c.o[t][r] = c.o[t][r] * e0 + y[(t * 16 + r) * 64] * e1;
         }
     }
-    store_part<DP, FULL>(a, c, l, p);
+    store_part<E, DP, FULL>(a, c, l, p);
     if constexpr (OWN)
-        if (any_bad) add_infinite<E, 32>(a, p);
+        if (any_bad) add_infinite<E, DP, 32>(a, p);
 }
 
 // The workgroups of the prefix, then those of the own keys.  Prefix: (head, row tile, split), the heads over
@@ -537,7 +563,15 @@ __device__ __forceinline__ bool find_part(const AttnArgs& a, bool own, uint32_t 
         p.sc = a.sc && p.valid ? a.sc + (((int64_t)b * a.Hkv + h) * R + mc) * a.tp : nullptr;
     }
     if (p.key1 > p.key0) return true;                      // (uniform over the workgroup)
-    if (p.valid && (threadIdx.x & 63) < 32) { a.pm[p.at] = -__builtin_inff(); a.pl[p.at] = 0.f; }
+    if (p.valid && (threadIdx.x & 63) < 32) {
+        if (a.whole) {
+            char* const out = out_row(a, p.at);
+            for (int d = 0; d < a.D; d += 8) *reinterpret_cast<v4u*>(out + 2 * d) = v4u{0, 0, 0, 0};
+        } else {
+            a.pm[p.at] = -__builtin_inff();
+            a.pl[p.at] = 0.f;
+        }
+    }
     return false;
 }
 
@@ -835,6 +869,7 @@ static void launch_all(const AttnArgs& a, const Plan& p, hipStream_t s) {
     if (p.np + p.no) segment_kernel<E, DP, FULL><<<(unsigned)(p.np + p.no), NW * 64, 0, s>>>(a);
     // threads a partial's row: by how many partials there are (at most 256 in all: D / 4 columns' threads)
     const int n = p.sp + p.ss;
+    if (a.whole) return;
     if (n > 8) launch_combine<E, 4>(a, p, s);
     else if (n > 2) launch_combine<E, 2>(a, p, s);
     else launch_combine<E, 1>(a, p, s);
@@ -919,6 +954,7 @@ extern "C" int otpu_attn_shared(const otpu_attn_args* args, otpu_stream_t stream
         if (p.scores) a.sc = f + p.sc;
         else a.lse = f + p.lse;
     }
+    a.whole = D <= 128 && p.sp + p.ss == 1 && !a.sc && !a.lse;
     const hipStream_t s = (hipStream_t)stream;
     if (dtype == OTPU_BF16) launch_type<BF16>(a, p, s);
     else launch_type<F16>(a, p, s);

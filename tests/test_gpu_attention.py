@@ -345,3 +345,32 @@ def test_many_small_weights(T):
             want = mass / (1 + mass)
             bound = want * (2.0 ** -11 + 2.0 ** -11 + 2.0 ** -12) + P * 2.0 ** -32 + 2.0 ** -25
             assert float((got - want).abs().max()) <= bound, (gap, place, float(got[0, 0, 0, 0]), want, bound)
+
+
+@pytest.mark.parametrize("dt", ["bfloat16", "float16"])
+def test_one_segment(T, dt):
+    """Where a row has one share and no weights are asked, it is stored as the output at once: the same bits as with
+    weights, whose call joins shares; into a view; rows that see nothing; infinities among newer tokens."""
+    from opentpu_amd import attention
+    rng = np.random.default_rng(23)
+    dt = getattr(T, dt)
+    for B, Lq, Hq, Hkv, D, P, Tn in ((3, 1, 4, 2, 128, 0, 40), (90, 1, 16, 8, 64, 0, 130), (2, 70, 8, 8, 96, 0, 200), (40, 100, 4, 4, 128, 0, 140),
+                                     (5, 1, 2, 1, 40, 60, 0), (300, 3, 16, 16, 128, 300, 0), (2, 3, 2, 2, 200, 0, 9)):
+        say("one segment", dt, B, Lq, Hq, Hkv, D, P, Tn)
+        args = [t.cuda() for t in make(T, rng, dt, B, Lq, Hq, Hkv, D, P, Tn)]
+        if Tn:
+            args[5][0], args[5][1] = 0, Tn
+            args[4][1, Tn - 1, :, 2] = float("inf")        # the newest token of sequence 1: seen by its last query
+        slab = T.full((B, Lq, Hq + 1, D + 8), 7.0, dtype=dt, device="cuda")
+        got = attention.shared(*args, out=slab[:, :, :Hq, :D])
+        if Tn:
+            want = attention.shared(*args, weights=T.zeros((B, Hkv, Tn), device="cuda"))
+            assert T.equal(got, want) and not got[0].any()
+            assert bool((got[1, -1, :, 2] == float("inf")).all()) and bool(T.isfinite(got[1, :-1]).all())
+        else:
+            own = [x.expand(B, *x.shape) for x in args[1:3]]   # the prefix as the caches of queries that see all of it
+            full = T.full((B,), P, dtype=T.int32, device="cuda")
+            for i in range(Lq):
+                want = attention.shared(args[0][:, i:i + 1], None, None, *own, full)
+                assert float((got[:, i:i + 1].float() - want.float()).abs().max()) <= 2 * 2.0 ** (-8 if dt == T.bfloat16 else -11) * 5
+        assert bool((slab[:, :, Hq:] == 7).all()) and bool((slab[..., D:] == 7).all())
