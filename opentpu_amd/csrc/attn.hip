@@ -57,6 +57,7 @@ struct AttnArgs {
     float scale2;                            // scale * log2(e)
     int sp, ss, per_p;                       // splits of the prefix, of the own keys; keys of a prefix split
     uint32_t np, no;                         // workgroups of the prefix, of the own keys
+    uint32_t half;                           // own keys: order of the row tiles (find_part), or 0
     int rows_p, rows_o;                      // rows of their tiles: 32 or 128
     bool whole;                              // one segment, D <= 128: a row's share is its output, nothing to join
     float* po;                               // partial o [sp + ss][rows][D]
@@ -522,7 +523,11 @@ __device__ __forceinline__ void keys_part(const AttnArgs& a, char* lds, const Pa
 // the XCDs and a split's row tiles next to each other, so that one L2 serves them the same keys.  (Both
 // kinds in turn, for the products of the one beside the loads of the other, takes that sharing from the
 // row tiles: 256 sequences on 131072 tokens 743 us, one kind after the other 526.)  Own: (head, row tile,
-// sequence, split).
+// sequence, split), without a prefix a sequence's last rows first: they see the most keys (64 x 512 queries on
+// their own 174 -> 171 us; behind a prefix no gain, and heads of 256 lose 2%).  Where a prompt's row tiles all have
+// their places at once and some CUs two, the first on the CUs (`half` a head) go from those of most keys
+// down and the second from the least up, so that each CU has the same work: 4096 queries on their own keys
+// 118 -> 104 us, 4 x 1024 42 -> 33.
 // The part of workgroup x of its kind; `wrow`: this lane's row in a tile of bm rows; false: no key
 __device__ __forceinline__ bool find_part(const AttnArgs& a, bool own, uint32_t x, int bm, int wrow, Part& p) {
     const int R = a.Lq * a.G;
@@ -545,7 +550,14 @@ __device__ __forceinline__ bool find_part(const AttnArgs& a, bool own, uint32_t 
         p.sc = nullptr;
     } else {
         const int tiles = (R + bm - 1) / bm;
-        const int tile = x % tiles, b = x / tiles % a.B, split = x / tiles / a.B;
+        int tile = x % tiles, b = x / tiles % a.B;
+        if (!a.np) tile = tiles - 1 - tile;
+        const int split = x / tiles / a.B;
+        if (a.half) {
+            const uint32_t k = x < a.half ? x : (uint32_t)tiles * a.B - 1 - (x - a.half);
+            tile = tiles - 1 - (int)(k / a.B);
+            b = k % a.B;
+        }
         const int mrow = tile * bm + wrow, mc = min(mrow, R - 1);
         const int i = mc / a.G, g = mc - i * a.G, head = h * a.G + g;
         const int len = min(max(a.lens[b], 0), a.T);
@@ -955,6 +967,8 @@ extern "C" int otpu_attn_shared(const otpu_attn_args* args, otpu_stream_t stream
         else a.lse = f + p.lse;
     }
     a.whole = D <= 128 && p.sp + p.ss == 1 && !a.sc && !a.lse;
+    const int cus = otpu_cu_count();
+    if (!p.np && p.ss == 1 && Lq > 1 && p.no > cus && p.no <= 2 * (int64_t)cus) a.half = (uint32_t)(cus / Hkv);
     const hipStream_t s = (hipStream_t)stream;
     if (dtype == OTPU_BF16) launch_type<BF16>(a, p, s);
     else launch_type<F16>(a, p, s);

@@ -374,3 +374,20 @@ def test_one_segment(T, dt):
                 want = attention.shared(args[0][:, i:i + 1], None, None, *own, full)
                 assert float((got[:, i:i + 1].float() - want.float()).abs().max()) <= 2 * 2.0 ** (-8 if dt == T.bfloat16 else -11) * 5
         assert bool((slab[:, :, Hq:] == 7).all()) and bool((slab[..., D:] == 7).all())
+
+
+def test_prompts_of_many_row_tiles(T):
+    """Prompts alone whose row tiles take each CU's first place and some of the second ones, in their own order: every
+    row of every sequence and head, the heads a divisor of the CUs and not."""
+    from opentpu_amd import attention
+    rng = np.random.default_rng(24)
+    for size in ((30, 150, 5, 5, 16, 0, 160), (18, 200, 8, 8, 16, 0, 210), (3, 290, 32, 16, 16, 0, 300)):
+        say("row tiles", size)
+        args = [t.cuda() for t in make(T, rng, T.bfloat16, *size)]
+        q, pk, pv, k, v, lens = args
+        lens[2] = size[6]
+        w0 = T.zeros((size[0], size[3], size[6]), device="cuda")
+        w = w0.clone()
+        got = attention.shared(q, None, None, k, v, lens, weights=w)
+        check(T, T.bfloat16, args, got, w0, w)
+        assert T.equal(attention.shared(q, None, None, k, v, lens), got)
