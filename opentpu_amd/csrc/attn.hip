@@ -384,7 +384,8 @@ __device__ __forceinline__ void clear_lds(char* lds, int bytes) {
 
 // Two workgroups a CU, a wave of each on a SIMD: the one's products fill the other's arithmetic in part (MFMA
 // busy 54% of the cycles at 1.9 GHz).  Two groups of waves that alternate at barriers instead, products beside
-// softmax: 780 TFLOP/s against 990.  Keys loaded two steps ahead: no change, the loads are not waited for.
+// softmax: 780 TFLOP/s against 990.  Keys loaded two steps ahead: no change, the loads are not waited for; four
+// places of 32 keys in place of two of 64: the same to 10% slower, for the barriers.
 template <class E, int DP, bool FULL, bool OWN>
 __device__ __forceinline__ void rows_part(const AttnArgs& a, char* lds, const Part& p) {
     using S = Shape<DP>;
