@@ -9,10 +9,10 @@
 //                         rows of k and v
 //   evict_move_kernel     more rows of k and v, and the slots that are free
 //
-// The moves are bound by memory (64 x 8 caches of 2048 slots cut to 1000: 268 MB read and written, 63 us with
-// the selection, 4.3 TB/s; a copy reaches 5.1).  The selection is a chain of a few trips to memory, three
+// The moves are bound by memory (64 x 8 caches of 2048 slots cut to 1000: 268 MB read and written, 64 us with
+// the selection, 4.2 TB/s; a copy reaches 5.1).  The selection is a chain of a few trips to memory, three
 // passes over keys in registers with three barriers each, and a scan: 8 us for 256 caches of 1024 slots with
-// the launch, 30 for caches of 32768, where one workgroup's instructions bound it.
+// the launch, 27 for caches of 32768, where one workgroup's instructions bound it.
 #include "otpu_common.h"
 
 namespace otpu {
