@@ -4,6 +4,7 @@
 // multiplied once by the rows of every sequence together and each sequence's cache by its own rows.
 //
 //   segment_kernel   one segment's share of the keys for a tile of rows: partial o, m, l
+//   both_kernel      all keys for a tile of rows, where such tiles fill the CUs
 //   combine_kernel   the partials of a row joined and rounded to the output's type; the own tokens'
 //                    weights from their scores
 //   weights_kernel   the weights where many rows would make the scores large: from the keys again
@@ -59,7 +60,8 @@ struct AttnArgs {
     uint32_t np, no;                         // workgroups of the prefix, of the own keys
     uint32_t half;                           // own keys: order of the row tiles (find_part), or 0
     int rows_p, rows_o;                      // rows of their tiles: 32 or 128
-    bool whole;                              // one segment, D <= 128: a row's share is its output, nothing to join
+    bool both;                               // a workgroup's rows against the prefix and their own keys (D <= 128)
+    bool whole;                              // a row's only share is its output, nothing to join (D <= 128)
     float* po;                               // partial o [sp + ss][rows][D]
     float* pm;                               // m [sp + ss][rows]
     float* pl;                               // l [sp + ss][rows]
@@ -277,6 +279,7 @@ struct Part {
     int64_t ks, vs;                          // byte strides of a token
     int key0, key1, lim;                     // lim: the segment's keys that this lane's row sees
     int least;                               // the least of the workgroup's rows
+    int head;                                // of the keys
     const char* q;                           // this lane's row
     bool valid;                              // a row of its own (not the clamped last one)
     int64_t at;                              // its place among the partials: (slot, row)
@@ -309,6 +312,7 @@ __device__ __forceinline__ void store_part(const AttnArgs& a, const Acc<DP>& c, 
     if (DP <= 128 && a.whole) {
         char* const out = out_row(a, p.at);
         const float il = l == 0.f ? 0.f : 1.f / l;
+        if (a.lse && hh == 0) a.lse[p.at] = c.m + __builtin_log2f(l);
 #pragma unroll
         for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
@@ -386,9 +390,12 @@ __device__ __forceinline__ void clear_lds(char* lds, int bytes) {
 // busy 54% of the cycles at 1.9 GHz).  Two groups of waves that alternate at barriers instead, products beside
 // softmax: 780 TFLOP/s against 990.  Keys loaded two steps ahead: no change, the loads are not waited for; four
 // places of 32 keys in place of two of 64: the same to 10% slower, for the barriers.
-template <class E, int DP, bool FULL, bool OWN>
+// BOTH: the prefix's keys, then the own ones (p's), as one row of steps.
+enum { PREFIX, OWN_KEYS, BOTH };
+template <class E, int DP, bool FULL, int KIND>
 __device__ __forceinline__ void rows_part(const AttnArgs& a, char* lds, const Part& p) {
     using S = Shape<DP>;
+    constexpr bool OWN = KIND != PREFIX;
     constexpr int KT = S::KT, CR = S::CR, LOADS = KT / (64 / CR) / NW;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Acc<DP> c;
@@ -397,12 +404,19 @@ __device__ __forceinline__ void rows_part(const AttnArgs& a, char* lds, const Pa
     v8s qf[DP / 16];
     load_query<DP, FULL>(qf, p.q, a.D);
     const uint32_t lds0 = lds_addr(lds);
-    const int n = p.key1 - p.key0, steps = (n + KT - 1) / KT;
+    const int before = KIND == BOTH ? (a.P + KT - 1) / KT : 0;   // steps of the prefix in front of the segment's own
+    const int n = p.key1 - p.key0, steps = before + (n + KT - 1) / KT;
     auto keys = [&](int i) INL {
-        load_rows<CR, FULL, false, KT, NW>(p.k, p.ks, p.key0 + i * KT, n - 1 - i * KT, lds0 + (uint32_t)((i & 1) * S::RB), wave, a.D);
+        const uint32_t to = lds0 + (uint32_t)((i & 1) * S::RB);
+        const bool own = KIND != BOTH || i >= before;
+        const int at = own ? p.key0 + (i - before) * KT : i * KT, end = own ? p.key1 : a.P;
+        load_rows<CR, FULL, false, KT, NW>(own ? p.k : a.pk + p.head * a.pkh, own ? p.ks : a.pks, at, end - 1 - at, to, wave, a.D);
     };
     auto vals = [&](int i) INL {
-        load_rows<CR, FULL, true, KT, NW>(p.v, p.vs, p.key0 + i * KT, n - 1 - i * KT, lds0 + (uint32_t)((2 + (i & 1)) * S::RB), wave, a.D);
+        const uint32_t to = lds0 + (uint32_t)((2 + (i & 1)) * S::RB);
+        const bool own = KIND != BOTH || i >= before;
+        const int at = own ? p.key0 + (i - before) * KT : i * KT, end = own ? p.key1 : a.P;
+        load_rows<CR, FULL, true, KT, NW>(own ? p.v : a.pv + p.head * a.pvh, own ? p.vs : a.pvs, at, end - 1 - at, to, wave, a.D);
     };
     keys(0);
     vals(0);
@@ -422,11 +436,12 @@ __device__ __forceinline__ void rows_part(const AttnArgs& a, char* lds, const Pa
         if (i + 1 < steps) vals(i + 1);
         if (i + 2 < steps) keys(i + 2);
         char* const vs = lds + (2 + (i & 1)) * S::RB;
-        const int at = p.key0 + i * KT;
-        if (OWN && at >= none) continue;                   // (uniform over the wave) no row of it sees these keys
-        raise(c, s, at, p.lim, first, a.scale2);
-        if (OWN && at + KT > p.least) bad |= finite_values<E>(vs, KT * CR);
-        if (!OWN && at + KT > p.key1) clear_tail<CR>(vs, p.key1 - at, KT);
+        const bool own = KIND == OWN_KEYS || (KIND == BOTH && i >= before);
+        const int at = KIND == BOTH && !own ? i * KT : p.key0 + (i - before) * KT, end = KIND == BOTH ? a.P : p.key1;
+        if (own && at >= none) continue;                   // (uniform over the wave) no row of it sees these keys
+        raise(c, s, at, KIND == BOTH && !own ? end : p.lim, KIND == BOTH && !own ? end : first, a.scale2);
+        if (own && at + KT > p.least) bad |= finite_values<E>(vs, KT * CR);
+        if (!own && at + KT > end) clear_tail<CR>(vs, end - at, KT);
         // the next scores' products among the weights' arithmetic (after the last step of a place's old keys, unused)
         scores<E, DP>(next, lds + ((i + 1) & 1) * S::RB, qf);
         weigh<E>(c, s, w, a.scale2);
@@ -533,7 +548,7 @@ __device__ __forceinline__ void keys_part(const AttnArgs& a, char* lds, const Pa
 __device__ __forceinline__ bool find_part(const AttnArgs& a, bool own, uint32_t x, int bm, int wrow, Part& p) {
     const int R = a.Lq * a.G;
     const int64_t rows = (int64_t)a.B * a.Lq * a.Hq;
-    const int h = x % a.Hkv;
+    const int h = p.head = x % a.Hkv;
     x /= a.Hkv;
     if (!own) {
         const int M = a.B * R, tiles = (M + bm - 1) / bm;
@@ -575,7 +590,7 @@ __device__ __forceinline__ bool find_part(const AttnArgs& a, bool own, uint32_t 
         p.at = (a.sp + split) * rows + ((int64_t)b * a.Lq + i) * a.Hq + head;
         p.sc = a.sc && p.valid ? a.sc + (((int64_t)b * a.Hkv + h) * R + mc) * a.tp : nullptr;
     }
-    if (p.key1 > p.key0) return true;                      // (uniform over the workgroup)
+    if (p.key1 > p.key0 || a.both) return true;            // (uniform over the workgroup)
     if (p.valid && (threadIdx.x & 63) < 32) {
         if (a.whole) {
             char* const out = out_row(a, p.at);
@@ -598,11 +613,22 @@ __global__ __launch_bounds__(NW * 64, DP <= 128 ? 2 : 1) void segment_kernel(Att
         return;
     if (!own) {
         if (keys) keys_part<E, DP, FULL, false>(a, lds, p);
-        else rows_part<E, DP, FULL, false>(a, lds, p);
+        else rows_part<E, DP, FULL, PREFIX>(a, lds, p);
     } else {
         if (keys) keys_part<E, DP, FULL, true>(a, lds, p);
-        else rows_part<E, DP, FULL, true>(a, lds, p);
+        else rows_part<E, DP, FULL, OWN_KEYS>(a, lds, p);
     }
+}
+
+// A sequence's tile of 128 rows against the prefix and its own keys (a kernel of its own: in segment_kernel its
+// addresses would not stay in scalar registers).  16 x 256 queries on 1024 shared tokens and their own, 16 heads
+// on 8 of 128: 76 -> 51 us; 4 x 2048 on 2048 274 -> 230, 8 x 512 on 8192 302 -> 291.
+template <class E, int DP, bool FULL>
+__global__ __launch_bounds__(NW * 64, 2) void both_kernel(AttnArgs a) {
+    __shared__ __attribute__((aligned(16))) char lds[Shape<DP>::ROWS_LDS];
+    Part p;
+    find_part(a, true, blockIdx.x, 32 * NW, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 32 + (threadIdx.x & 31), p);
+    rows_part<E, DP, FULL, BOTH>(a, lds, p);
 }
 
 // The partials of a row joined: GP threads take every GP-th partial of four columns, their sums meet in
@@ -817,6 +843,7 @@ struct Plan {
     int sp, ss, per_p;                       // splits; keys of a prefix split
     int64_t np, no;                          // workgroups
     int64_t rows, tp;
+    bool both;                               // one segment of the prefix and the own keys
     bool scores;                             // own scores kept for the weights
     int64_t po, pm, pl, lse, sc, bytes;      // the work area's parts, in floats; its size
 };
@@ -853,6 +880,13 @@ static Plan plan(int B, int Lq, int Hq, int Hkv, int D, int P, int T) {
     p.sp = (int)s;
     p.per_p = p.sp ? ((P + p.sp - 1) / p.sp + 31) & ~31 : 0;
     p.np = gp * p.sp;
+    // Tiles of a sequence's rows that fill the places take the prefix and their own keys in one: no partials, no
+    // join.  Where sequences leave little of their last tiles free (1 in 20 rows at most).
+    p.both = D <= 128 && p.sp == 1 && p.ss == 1 && p.rows_o == 128 && 20 * 128 * (go / Hkv) <= 21 * M;
+    if (p.both) {
+        p.sp = 0;
+        p.np = 0;
+    }
     p.scores = R <= 32;
     p.tp = (T + 31) & ~31;
     const int64_t n = p.sp + p.ss;
@@ -879,11 +913,13 @@ static void launch_combine(const AttnArgs& a, const Plan& p, hipStream_t s) {
 
 template <class E, int DP, bool FULL>
 static void launch_all(const AttnArgs& a, const Plan& p, hipStream_t s) {
-    if (p.np + p.no) segment_kernel<E, DP, FULL><<<(unsigned)(p.np + p.no), NW * 64, 0, s>>>(a);
+    if constexpr (DP <= 128)
+        if (a.both) both_kernel<E, DP, FULL><<<(unsigned)p.no, NW * 64, 0, s>>>(a);
+    if (!a.both && p.np + p.no) segment_kernel<E, DP, FULL><<<(unsigned)(p.np + p.no), NW * 64, 0, s>>>(a);
     // threads a partial's row: by how many partials there are (at most 256 in all: D / 4 columns' threads)
     const int n = p.sp + p.ss;
-    if (a.whole) return;
-    if (n > 8) launch_combine<E, 4>(a, p, s);
+    if (a.whole) {}
+    else if (n > 8) launch_combine<E, 4>(a, p, s);
     else if (n > 2) launch_combine<E, 2>(a, p, s);
     else launch_combine<E, 1>(a, p, s);
     if (a.weights && a.T && !a.sc)
@@ -967,7 +1003,8 @@ extern "C" int otpu_attn_shared(const otpu_attn_args* args, otpu_stream_t stream
         if (p.scores) a.sc = f + p.sc;
         else a.lse = f + p.lse;
     }
-    a.whole = D <= 128 && p.sp + p.ss == 1 && !a.sc && !a.lse;
+    a.both = p.both;
+    a.whole = p.both || (D <= 128 && p.sp + p.ss == 1 && !a.sc);
     const int cus = otpu_cu_count();
     if (!p.np && p.ss == 1 && Lq > 1 && p.no > cus && p.no <= 2 * (int64_t)cus) a.half = (uint32_t)(cus / Hkv);
     const hipStream_t s = (hipStream_t)stream;

@@ -391,3 +391,40 @@ def test_prompts_of_many_row_tiles(T):
         got = attention.shared(q, None, None, k, v, lens, weights=w)
         check(T, T.bfloat16, args, got, w0, w)
         assert T.equal(attention.shared(q, None, None, k, v, lens), got)
+
+
+@pytest.mark.parametrize("dt", ["bfloat16", "float16"])
+def test_prefix_and_own_keys_in_one(T, dt):
+    """Queries of a tile's size and more on a short prefix: a workgroup takes the prefix and its sequence's keys.  Lengths
+    of 0, below the queries' number and full; infinities at the prefix's end, NaN past lens and in newer tokens."""
+    from opentpu_amd import attention
+    rng = np.random.default_rng(25)
+    dt = getattr(T, dt)
+    nan, inf = float("nan"), float("inf")
+    for size in ((13, 125, 4, 4, 16, 100, 150), (3, 128, 2, 2, 128, 64, 140), (3, 64, 4, 2, 64, 7, 200), (3, 128, 2, 1, 96, 33, 256),
+                 (3, 128, 1, 1, 128, 1, 128)):
+        say("both", dt, size)
+        B, Lq, Hq, Hkv, D, P, Tn = size
+        args = [t.cuda() for t in make(T, rng, dt, *size)]
+        q, pk, pv, k, v, lens = args
+        lens[0], lens[1], lens[2] = 0, Tn, Lq // 2
+        w0 = T.from_numpy(rng.random((B, Hkv, Tn)).astype(np.float32)).cuda()
+        w = w0.clone()
+        got = attention.shared(*args, weights=w)
+        check(T, dt, args, got, w0, w)
+        assert T.equal(attention.shared(*args), got)
+        # what a query does not see
+        for b in range(B):
+            k[b, int(lens[b]):], v[b, int(lens[b]):] = nan, (nan, inf, -inf)[b % 3]
+        assert T.equal(attention.shared(*args), got)
+        k[1, Tn - 1, :, 0], v[1, Tn - 1, :, 1] = nan, inf
+        new = attention.shared(*args)
+        assert T.equal(new[0], got[0]) and T.equal(new[1, :-1], got[1, :-1]) and bool(T.isnan(new[1, -1]).all())
+        # what every query sees
+        k[1, Tn - 1, :, 0], v[1, Tn - 1, :, 1] = 0.5, 1.0
+        pv[P - 1, :, 3], pv[P - 1, :, 4] = inf, -inf
+        new = attention.shared(*args)
+        assert bool((new[..., 3] == inf).all()) and bool((new[..., 4] == -inf).all()) and bool(T.isfinite(new[..., 5:]).all())
+        q[1, 0, 0, 0] = nan
+        new2 = attention.shared(*args)
+        assert bool(T.isnan(new2[1, 0, 0]).all()) and T.equal(new2[1, 1:], new[1, 1:]) and T.equal(new2[0], new[0])
