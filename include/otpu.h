@@ -404,7 +404,9 @@ int otpu_norm_qact(const void* x, int64_t ldx, const void* res, int64_t ldr, int
  *   weights fp32.  D a multiple of 8, at most 256; scale > 0; addresses 16-byte aligned, strides
  *   multiples of 8, tokens less than 2^22 elements apart.  P and T at most 2^30, either may
  *   be 0 (its operands NULL).
- *   work: otpu_attn_work_bytes(...) bytes, 256-byte aligned, free again when the call's kernels ended.
+ *   work: 256-byte aligned, free again when the call's kernels ended.  work_bytes is otpu_attn_work_bytes(...)
+ *   or more, which serves every call of these sizes, or exactly otpu_attn_call_bytes(...): what a call with
+ *   weights, or without, uses (0 where each row is stored as it is computed; work may then be NULL).
  *   The arguments come as a struct on the host, read before the call returns. */
 typedef struct otpu_attn_args {
     int64_t bytes;                                    /* sizeof(otpu_attn_args) */
@@ -421,6 +423,7 @@ typedef struct otpu_attn_args {
     double scale;
 } otpu_attn_args;
 int64_t otpu_attn_work_bytes(int B, int Lq, int Hq, int Hkv, int D, int P, int T);
+int64_t otpu_attn_call_bytes(int B, int Lq, int Hq, int Hkv, int D, int P, int T, int weights);
 int otpu_attn_shared(const otpu_attn_args* args, otpu_stream_t stream);
 
 /* Eviction from a cache by accumulated attention weight: where lens[b] > budget, each head keeps `budget`

@@ -66,6 +66,7 @@ SIGNATURES = {
     "otpu_mx_matmul": ([_P, _L, _P, _L, _P, _L, _P, _L, _I, _I, _I, _I, _I, _P, _L, _P], _I),
     "otpu_norm_qact": ([_P, _L, _P, _L, _I, _I, _I, _P, _F, _I, _P, _L, _P, _P, _L, _P, _P, _L, _P], _I),
     "otpu_attn_work_bytes": ([_I, _I, _I, _I, _I, _I, _I], _L),
+    "otpu_attn_call_bytes": ([_I, _I, _I, _I, _I, _I, _I, _I], _L),
     "otpu_attn_shared": ([C.c_char_p, _P], _I),
     "otpu_kv_evict_work_bytes": ([_I, _I, _I, _I], _L),
     "otpu_kv_evict": ([C.c_char_p, _P], _I),

@@ -23,7 +23,7 @@ def _types():
 
 @functools.lru_cache(maxsize=1024)
 def _attn_bytes(*sizes) -> int:
-    return X.load().otpu_attn_work_bytes(*sizes)
+    return X.load().otpu_attn_call_bytes(*sizes)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -109,7 +109,7 @@ def shared(q, prefix_k, prefix_v, k, v, lens, *, scale: float | None = None, wei
         os = _rows("shared", "out", out, dt, (B, Lq, Hq, D), dev, True)
     if out.numel() == 0:
         return out
-    nbytes = _attn_bytes(B, Lq, Hq, Hkv, D, P, N)
+    nbytes = _attn_bytes(B, Lq, Hq, Hkv, D, P, N, weights is not None)
     work = q.new_empty((nbytes // 2 + 1,))                 # (of q's type: the least work for the host)
     X.call("otpu_attn_shared", X.ATTN_ARGS.pack(
         X.ATTN_ARGS.size, q.data_ptr(), qs[0], qs[1], qs[2], pk, ps[0], ps[1], pv, pvs[0], pvs[1], kp, ks[0], ks[1], ks[2], vp,

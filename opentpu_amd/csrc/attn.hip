@@ -844,11 +844,13 @@ struct Plan {
     int64_t np, no;                          // workgroups
     int64_t rows, tp;
     bool both;                               // one segment of the prefix and the own keys
+    bool whole;                              // one share a row, stored as its output
     bool scores;                             // own scores kept for the weights
     int64_t po, pm, pl, lse, sc, bytes;      // the work area's parts, in floats; its size
 };
 
-static Plan plan(int B, int Lq, int Hq, int Hkv, int D, int P, int T) {
+// weights: the call asks for them.  any: the parts that some call of these sizes uses.
+static Plan plan(int B, int Lq, int Hq, int Hkv, int D, int P, int T, bool weights, bool any = false) {
     Plan p = {};
     const int R = Lq * (Hq / Hkv);
     const int64_t M = (int64_t)B * R, slots = 2 * (int64_t)otpu_cu_count();
@@ -887,9 +889,10 @@ static Plan plan(int B, int Lq, int Hq, int Hkv, int D, int P, int T) {
         p.sp = 0;
         p.np = 0;
     }
-    p.scores = R <= 32;
+    p.scores = weights && T && R <= 32;
+    p.whole = p.both || (D <= 128 && p.sp + p.ss == 1 && !p.scores);
     p.tp = (T + 31) & ~31;
-    const int64_t n = p.sp + p.ss;
+    const int64_t n = p.whole && !any ? 0 : p.sp + p.ss;   // partials
     auto part = [&](int64_t floats) {
         const int64_t at = p.bytes / 4;
         p.bytes += (4 * floats + 255) & ~(int64_t)255;
@@ -898,8 +901,8 @@ static Plan plan(int B, int Lq, int Hq, int Hkv, int D, int P, int T) {
     p.po = part(n * p.rows * D);
     p.pm = part(n * p.rows);
     p.pl = part(n * p.rows);
-    p.lse = part(p.rows);
-    p.sc = part(p.scores ? (int64_t)B * Hkv * R * p.tp : 0);
+    p.lse = part(any || (weights && T && !p.scores) ? p.rows : 0);
+    p.sc = part(p.scores || (any && R <= 32) ? (int64_t)B * Hkv * R * p.tp : 0);
     return p;
 }
 
@@ -954,7 +957,12 @@ static int check_sizes(const char* who, int B, int Lq, int Hq, int Hkv, int D, i
 
 extern "C" int64_t otpu_attn_work_bytes(int B, int Lq, int Hq, int Hkv, int D, int P, int T) {
     if (check_sizes("attn_work_bytes", B, Lq, Hq, Hkv, D, P, T)) return -1;
-    return plan(B, Lq, Hq, Hkv, D, P, T).bytes;
+    return plan(B, Lq, Hq, Hkv, D, P, T, false, true).bytes;
+}
+
+extern "C" int64_t otpu_attn_call_bytes(int B, int Lq, int Hq, int Hkv, int D, int P, int T, int weights) {
+    if (check_sizes("attn_call_bytes", B, Lq, Hq, Hkv, D, P, T)) return -1;
+    return plan(B, Lq, Hq, Hkv, D, P, T, weights != 0).bytes;
 }
 
 extern "C" int otpu_attn_shared(const otpu_attn_args* args, otpu_stream_t stream) {
@@ -966,7 +974,8 @@ extern "C" int otpu_attn_shared(const otpu_attn_args* args, otpu_stream_t stream
     if (const int rc = check_sizes("attn_shared", B, Lq, Hq, Hkv, D, P, T)) return rc;
     if (!(scale > 0.) || scale > 1e30) return otpu_fail(OTPU_EINVAL, "attn_shared: scale %g", scale);
     if (B == 0 || Lq == 0) return OTPU_OK;
-    if (!q || !out || !work || (P && (!pk || !pv)) || (T && (!k || !v || !lens)))
+    const Plan p = plan(B, Lq, Hq, Hkv, D, P, T, weights != nullptr);
+    if (!q || !out || (!work && (p.bytes || work_bytes)) || (P && (!pk || !pv)) || (T && (!k || !v || !lens)))
         return otpu_fail(OTPU_EINVAL, "attn_shared: a NULL operand");
     const int64_t st[] = {qb, qt, qh, P ? pks : 0, P ? pkh : 0, P ? pvs : 0, P ? pvh : 0, T ? kb : 0, T ? kt : 0,
                           T ? kh : 0, T ? vb : 0, T ? vt : 0, T ? vh : 0, ob, ot, oh};
@@ -978,10 +987,12 @@ extern "C" int otpu_attn_shared(const otpu_attn_args* args, otpu_stream_t stream
     if (!al16(q) || !al16(out) || (P && (!al16(pk) || !al16(pv))) || (T && (!al16(k) || !al16(v))) ||
         ((uintptr_t)work & 255) || (T && ((uintptr_t)lens & 3)) || ((uintptr_t)weights & 3))
         return otpu_fail(OTPU_EALIGN, "attn_shared: operands 16-byte aligned, work 256-byte");
-    const Plan p = plan(B, Lq, Hq, Hkv, D, P, T);
-    if (work_bytes < p.bytes)
-        return otpu_fail(OTPU_EINVAL, "attn_shared: work area of %lld bytes, need %lld", (long long)work_bytes,
-                         (long long)p.bytes);
+    if (work_bytes != p.bytes) {
+        const int64_t any = plan(B, Lq, Hq, Hkv, D, P, T, false, true).bytes;
+        if (work_bytes < any)
+            return otpu_fail(OTPU_EINVAL, "attn_shared: work area of %lld bytes, need %lld, or this call's %lld", (long long)work_bytes,
+                             (long long)any, (long long)p.bytes);
+    }
     AttnArgs a = {};
     a.q = (const char*)q; a.qb = 2 * qb; a.qt = 2 * qt; a.qh = 2 * qh;
     a.pk = (const char*)pk; a.pks = 2 * pks; a.pkh = 2 * pkh;
@@ -1004,7 +1015,7 @@ extern "C" int otpu_attn_shared(const otpu_attn_args* args, otpu_stream_t stream
         else a.lse = f + p.lse;
     }
     a.both = p.both;
-    a.whole = p.both || (D <= 128 && p.sp + p.ss == 1 && !a.sc);
+    a.whole = p.whole;
     const int cus = otpu_cu_count();
     if (!p.np && p.ss == 1 && Lq > 1 && p.no > cus && p.no <= 2 * (int64_t)cus) a.half = (uint32_t)(cus / Hkv);
     const hipStream_t s = (hipStream_t)stream;
