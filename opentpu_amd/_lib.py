@@ -137,6 +137,14 @@ def stream():
     return C.c_void_p(T._C._cuda_getCurrentRawStream(T.cuda.current_device()))
 
 
+def stream_of(who: str, dev: int):
+    """stream() for a call whose tensors are on device `dev`: it has to be the current one, whose stream that is."""
+    T = _T or torch()
+    if dev != T.cuda.current_device():
+        raise ValueError(f"{who}: tensors on cuda:{dev}, the current device is cuda:{T.cuda.current_device()}")
+    return C.c_void_p(T._C._cuda_getCurrentRawStream(dev))
+
+
 def ptr(t):
     return C.c_void_p(t.data_ptr()) if t is not None else None
 

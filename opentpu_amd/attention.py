@@ -3,7 +3,7 @@ reads: `shared` (the prefix's keys and values multiplied once by the queries of 
 sequence's own cache by its own, one softmax over both) and `evict` (slots of the own caches freed by
 accumulated attention weight).
 
-Device tensors, bfloat16 or float16; every call is queued on the current torch stream and allocates its
+Tensors of the current device, bfloat16 or float16; every call is queued on the current torch stream and allocates its
 work area from torch's allocator on that stream."""
 from __future__ import annotations
 
@@ -114,7 +114,7 @@ def shared(q, prefix_k, prefix_v, k, v, lens, *, scale: float | None = None, wei
     X.call("otpu_attn_shared", X.ATTN_ARGS.pack(
         X.ATTN_ARGS.size, q.data_ptr(), qs[0], qs[1], qs[2], pk, ps[0], ps[1], pv, pvs[0], pvs[1], kp, ks[0], ks[1], ks[2], vp,
         vs[0], vs[1], vs[2], lp, out.data_ptr(), os[0], os[1], os[2], wp, work.data_ptr(), nbytes, B, Lq, Hq, Hkv, D, P, N,
-        kinds[dt], D ** -0.5 if scale is None else scale), X.stream())
+        kinds[dt], D ** -0.5 if scale is None else scale), X.stream_of("shared", dev))
     return out
 
 
@@ -150,7 +150,7 @@ def evict(k, v, weights, pos, lens, budget: int, recent: int = 0, *, out=None):
     work = lens.new_empty((nbytes // 4 + 1,))
     X.call("otpu_kv_evict", X.EVICT_ARGS.pack(
         X.EVICT_ARGS.size, k.data_ptr(), e * ks[0], e * ks[1], e * ks[2], v.data_ptr(), e * vs[0], e * vs[1], e * vs[2], *address,
-        work.data_ptr(), nbytes, B, N, H, e * D, budget, recent), X.stream())
+        work.data_ptr(), nbytes, B, N, H, e * D, budget, recent), X.stream_of("evict", dev))
     return out
 
 

@@ -216,7 +216,7 @@ def norm_quantize(x, gamma, residual=None, *, eps: float = 1e-6, row_mode: bool 
     `dot` (an offset a group of 32; row_mode: one): as `fp32.qact` of the fp32 h with rscale r and cscale
     gamma.  x [M, K] float32, bfloat16 or float16, residual of its type (or None), gamma [K]; K a multiple
     of 32 (a `dot` needs 128).  Returns (operand, h): h in x's type, x itself without a residual.
-    h: a tensor for the sum, x or residual among them; r: a float32 tensor [M] for the rows' factors."""
+    Tensors of the current device.  h: a tensor for the sum, x or residual among them; r: a float32 tensor [M] for the rows' factors."""
     T = X.torch()
     if not NORM_TYPES:
         NORM_TYPES.update({T.float32: X.F32, T.bfloat16: X.BF16, T.float16: X.F16})
@@ -250,7 +250,8 @@ def norm_quantize(x, gamma, residual=None, *, eps: float = 1e-6, row_mode: bool 
     S = gamma.new_empty((1, M))
     d = q.new_empty((M, K // 32), dtype=T.uint8)
     X.call("otpu_norm_qact", x.data_ptr(), xs[0], rp, rs, NORM_TYPES[dt], M, K, gamma.data_ptr(), eps,
-           X.Q_ROW if row_mode else 0, hp, hs, None if r is None else r.data_ptr(), q.data_ptr(), K, S.data_ptr(), d.data_ptr(), K // 32, X.stream())
+           X.Q_ROW if row_mode else 0, hp, hs, None if r is None else r.data_ptr(), q.data_ptr(), K, S.data_ptr(), d.data_ptr(), K // 32,
+           X.stream_of("norm_quantize", dev))
     return _operand(q, S, d, [K], bool(row_mode)), x if h is None else h
 
 
