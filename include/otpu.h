@@ -401,7 +401,7 @@ int otpu_norm_qact(const void* x, int64_t ldx, const void* res, int64_t ldr, int
  *   out [B, Lq, Hq, D] = sum softmax(scale q k) v; 0 where a query sees no key.  weights (may be NULL)
  *   [B, Hkv, T] fp32: the own tokens' softmax weights, summed over the Lq queries and the head's Hq / Hkv
  *   query heads, are added to it.  dtype OTPU_BF16 or OTPU_F16 for q, caches and out; sums, maxima and
- *   weights fp32.  D a multiple of 8, at most 256; scale > 0; addresses 16-byte aligned, strides
+ *   weights fp32.  D a multiple of 8, at most 256; scale from 5e-46 to 1e30; addresses 16-byte aligned, strides
  *   multiples of 8, tokens less than 2^22 elements apart.  P and T at most 2^30, either may
  *   be 0 (its operands NULL).
  *   work: 256-byte aligned, free again when the call's kernels ended.  work_bytes is otpu_attn_work_bytes(...)

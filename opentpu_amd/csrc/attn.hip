@@ -972,7 +972,9 @@ extern "C" int otpu_attn_shared(const otpu_attn_args* args, otpu_stream_t stream
                 work, work_bytes, B, Lq, Hq, Hkv, D, P, T, dtype, scale] = *args;
     if (dtype != OTPU_BF16 && dtype != OTPU_F16) return otpu_fail(OTPU_EFORMAT, "attn_shared: type %d (bf16, fp16)", dtype);
     if (const int rc = check_sizes("attn_shared", B, Lq, Hq, Hkv, D, P, T)) return rc;
-    if (!(scale > 0.) || scale > 1e30) return otpu_fail(OTPU_EINVAL, "attn_shared: scale %g", scale);
+    // (0 in fp32 would make NaN of the keys that a row does not see)
+    const float scale2 = (float)(scale * 1.4426950408889634);
+    if (!(scale2 > 0.f) || scale > 1e30) return otpu_fail(OTPU_EINVAL, "attn_shared: scale %g", scale);
     if (B == 0 || Lq == 0) return OTPU_OK;
     const Plan p = plan(B, Lq, Hq, Hkv, D, P, T, weights != nullptr);
     if (!q || !out || (!work && (p.bytes || work_bytes)) || (P && (!pk || !pv)) || (T && (!k || !v || !lens)))
@@ -1003,7 +1005,7 @@ extern "C" int otpu_attn_shared(const otpu_attn_args* args, otpu_stream_t stream
     a.out = (char*)out; a.ob = 2 * ob; a.ot = 2 * ot; a.oh = 2 * oh;
     a.weights = weights;
     a.P = P; a.T = T; a.B = B; a.Lq = Lq; a.Hq = Hq; a.Hkv = Hkv; a.G = Hq / Hkv; a.D = D;
-    a.scale2 = (float)(scale * 1.4426950408889634);
+    a.scale2 = scale2;
     a.sp = p.sp; a.ss = p.ss; a.per_p = p.per_p;
     a.np = (uint32_t)p.np; a.no = (uint32_t)p.no;
     a.rows_p = p.rows_p; a.rows_o = p.rows_o;
