@@ -130,12 +130,16 @@ class Batch:
         return (y + h).view(B, L, s.hidden)
 
     def step(self, x):
-        """The next L tokens of every sequence, x [B, L, hidden] float32 -> [B, L, hidden]."""
+        """The next L tokens of every sequence, x [B, L, hidden] float32 -> [B, L, hidden].  L is at most the slots
+        over the budget, or those that are free."""
+        if x.dim() != 3 or x.shape[0] != self.B or x.shape[2] != self.shape.hidden:
+            raise ValueError(f"step: x is {list(x.shape)}, needs [{self.B}, L, {self.shape.hidden}]")
         L = x.shape[1]
         if self.used + L > self.slots:
+            kept = min(self.used, self.budget)
+            if kept + L > self.slots:                      # (refused before anything is evicted)
+                raise ValueError(f"step: {L} tokens after {kept} in {self.slots} slots")
             self.evict()
-        if self.used + L > self.slots:
-            raise ValueError(f"step: {L} tokens after {self.used} in {self.slots} slots")
         n, at = self.used, self.position
         self.lens.fill_(n + L)
         T = X.torch()
