@@ -56,6 +56,11 @@ def _rows(who: str, name: str, t, dtype, shape, dev: int, written: bool = False)
     return s
 
 
+def _used(shape, s) -> tuple:
+    """Strides, 0 for dimensions of one place: no address has them in it, so they may be anything."""
+    return tuple(0 if n == 1 else x for n, x in zip(shape, s))
+
+
 def shared(q, prefix_k, prefix_v, k, v, lens, *, scale: float | None = None, weights=None, out=None):
     """Attention of q [B, Lq, Hq, D] over the shared prefix [P, Hkv, D] and each sequence's own cache
     k, v [B, T, Hkv, D], of which lens [B] (int32) tokens are in use, the Lq newest the queries' own:
@@ -109,6 +114,10 @@ def shared(q, prefix_k, prefix_v, k, v, lens, *, scale: float | None = None, wei
         os = _rows("shared", "out", out, dt, (B, Lq, Hq, D), dev, True)
     if out.numel() == 0:
         return out
+    if N == 1 or P == 1 or (qs[0] | qs[1] | qs[2] | ps[0] | ps[1] | pvs[0] | pvs[1] | ks[0] | ks[1] | ks[2] | vs[0] | vs[1] | vs[2]
+                            | os[0] | os[1] | os[2]) & 7:
+        qs, os, own, pre = _used(q.shape, qs), _used(q.shape, os), (B, N, Hkv), (P, Hkv)
+        ks, vs, ps, pvs = _used(own, ks), _used(own, vs), _used(pre, ps), _used(pre, pvs)
     nbytes = _attn_bytes(B, Lq, Hq, Hkv, D, P, N, weights is not None)
     work = q.new_empty((nbytes // 2 + 1,))                 # (of q's type: the least work for the host)
     X.call("otpu_attn_shared", X.ATTN_ARGS.pack(
@@ -133,7 +142,7 @@ def evict(k, v, weights, pos, lens, budget: int, recent: int = 0, *, out=None):
         raise ValueError(f"evict: k is {dt} {list(k.shape)} on {k.device}, needs [B, T, H, D] in bfloat16, float16 or float32")
     B, N, H, D = k.shape
     e = k.element_size()
-    ks, vs = _rows("evict", "k", k, dt, (B, N, H, D), dev, True), _rows("evict", "v", v, dt, (B, N, H, D), dev, True)
+    ks, vs = (_used(k.shape, _rows("evict", name, t, dt, (B, N, H, D), dev, True)) for name, t in (("k", k), ("v", v)))
     slots = (B, H, N)
     if out is None:
         out = (T.empty_like(weights), T.empty_like(pos), T.empty_like(lens))

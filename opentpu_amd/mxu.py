@@ -246,10 +246,11 @@ def norm_quantize(x, gamma, residual=None, *, eps: float = 1e-6, row_mode: bool 
             raise _norm_refusal("h", h, x)
     if r is not None and (r.dtype != T.float32 or r.shape != (M,) or not r.is_contiguous() or r.get_device() != dev):
         raise ValueError("norm_quantize: r is a contiguous float32 tensor [M]")
+    xs, rs, hs = (xs[0], rs, hs) if M > 1 else (K, K, K)   # (one row: its stride may be anything)
     q = T.empty_like(x, dtype=T.int8, memory_format=T.contiguous_format)
     S = gamma.new_empty((1, M))
     d = q.new_empty((M, K // 32), dtype=T.uint8)
-    X.call("otpu_norm_qact", x.data_ptr(), xs[0], rp, rs, NORM_TYPES[dt], M, K, gamma.data_ptr(), eps,
+    X.call("otpu_norm_qact", x.data_ptr(), xs, rp, rs, NORM_TYPES[dt], M, K, gamma.data_ptr(), eps,
            X.Q_ROW if row_mode else 0, hp, hs, None if r is None else r.data_ptr(), q.data_ptr(), K, S.data_ptr(), d.data_ptr(), K // 32,
            X.stream_of("norm_quantize", dev))
     return _operand(q, S, d, [K], bool(row_mode)), x if h is None else h
