@@ -8,6 +8,7 @@ work area from torch's allocator on that stream."""
 from __future__ import annotations
 
 import functools
+import operator
 
 from . import _lib as X
 
@@ -54,6 +55,11 @@ def _rows(who: str, name: str, t, dtype, shape, dev: int, written: bool = False)
     if s[-1] != 1 and t.numel() and shape[-1] > 1:
         raise ValueError(f"{who}: the columns of {name} must be adjacent")
     return s
+
+
+def _count(x) -> int:
+    """A whole number as the ABI's int32: more slots than any cache has, or fewer than none, stay that."""
+    return max(-1, min(operator.index(x), 0x7FFFFFFF))
 
 
 def _used(shape, s) -> tuple:
@@ -138,6 +144,7 @@ def evict(k, v, weights, pos, lens, budget: int, recent: int = 0, *, out=None):
     length have weight 0 and position -1.  out: the three tensors to write them to; (weights, pos, lens)
     themselves may be given."""
     dt, dev, T = k.dtype, k.get_device(), X.torch()
+    budget, recent = _count(budget), _count(recent)
     if k.dim() != 4 or dev < 0 or dt not in _types():
         raise ValueError(f"evict: k is {dt} {list(k.shape)} on {k.device}, needs [B, T, H, D] in bfloat16, float16 or float32")
     B, N, H, D = k.shape
