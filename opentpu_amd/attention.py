@@ -92,6 +92,8 @@ def shared(q, prefix_k, prefix_v, k, v, lens, *, scale: float | None = None, wei
     qs = q.stride()
     if qs[3] != 1:
         _rows("shared", "q", q, dt, (B, Lq, Hq, D), dev)
+    if (k is not None and k.dim() != 4) or (prefix_k is not None and prefix_k.dim() != 3):
+        raise ValueError("shared: a cache has four dimensions, a prefix three")
     if k is not None:                                      # (tests in line: the functions say what is wrong)
         N, Hkv = k.shape[1], k.shape[-2]
         own, ks, vs = (B, N, Hkv, D), k.stride(), v.stride()

@@ -40,3 +40,21 @@ def test_budget_and_recent_past_32_bits(T):
     for bad in ((5.0, 0), (5, 1.5), ("5", 0)):
         with pytest.raises(TypeError):
             run(*bad)
+
+
+def test_other_ranks(T):
+    from opentpu_amd import attention
+    q, p, k = T.zeros((2, 1, 4, 64), device="cuda").half(), T.zeros((5, 2, 64), device="cuda").half(), T.zeros((2, 7, 2, 64), device="cuda").half()
+    lens = T.zeros((2,), dtype=T.int32, device="cuda")
+    flat, one = T.zeros((64,), device="cuda").half(), T.zeros((), device="cuda").half()
+    for x in (flat, one, k[0], p[0]):
+        for bad in (lambda: attention.shared(q, None, None, x, x, lens), lambda: attention.shared(q, p, p, x, k, lens),
+                    lambda: attention.shared(q, p, p, k, x, lens), lambda: attention.shared(q, p, p, k, k, x),
+                    lambda: attention.evict(k, x, T.zeros((2, 2, 7), device="cuda"), lens, lens, 3)):
+            with pytest.raises(ValueError):
+                bad()
+    for x in (flat, one, k, p[0]):
+        for bad in (lambda: attention.shared(q, x, x, None, None, None), lambda: attention.shared(q, x, p, k, k, lens),
+                    lambda: attention.shared(q, p, x, k, k, lens)):
+            with pytest.raises(ValueError):
+                bad()
