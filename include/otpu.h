@@ -386,7 +386,7 @@ enum { OTPU_F32 = 0, OTPU_BF16 = 1, OTPU_F16 = 2 };
  *   cscale gamma quantizes the fp32 h, bit for bit.
  *   x [M, ldx], res [M, ldr], h [M, ldh] of type dtype (OTPU_F32, OTPU_BF16, OTPU_F16); h (may be NULL)
  *   gets the sum rounded to dtype and may be x or res; gamma [K] fp32; r [M] (may be NULL); q, S, d as
- *   otpu_qact.  K a multiple of 32, at most OTPU_NORM_COLS.  Rows 16-byte aligned; q's rows 4-byte (16-bit
+ *   otpu_qact.  K a multiple of 32, at most OTPU_NORM_COLS, M below 2^22.  Rows 16-byte aligned; q's rows 4-byte (16-bit
  *   types: 8-byte) aligned.  A row whose sum of squares passes fp32's range gives r = 0. */
 #define OTPU_NORM_COLS 32768
 int otpu_norm_qact(const void* x, int64_t ldx, const void* res, int64_t ldr, int dtype, int M, int K,
@@ -402,8 +402,9 @@ int otpu_norm_qact(const void* x, int64_t ldx, const void* res, int64_t ldr, int
  *   [B, Hkv, T] fp32: the own tokens' softmax weights, summed over the Lq queries and the head's Hq / Hkv
  *   query heads, are added to it.  dtype OTPU_BF16 or OTPU_F16 for q, caches and out; sums, maxima and
  *   weights fp32.  D a multiple of 8, at most 256; scale from 5e-46 to 1e30; addresses 16-byte aligned, strides
- *   multiples of 8, tokens less than 2^22 elements apart.  P and T at most 2^30, either may
- *   be 0 (its operands NULL).
+ *   multiples of 8, tokens less than 2^22 elements apart.  P or T may be 0 (its operands NULL).
+ *   Limits: B * Lq * Hq at most 2^23 rows, P at most 2^30, B * Hkv * ceil(T / 32) below 2^24 (one cache of
+ *   2^29 - 32 tokens; 256 sequences on 8 heads of 262112).
  *   work: 256-byte aligned, free again when the call's kernels ended.  work_bytes is otpu_attn_work_bytes(...)
  *   or more, which serves every call of these sizes, or exactly otpu_attn_call_bytes(...): what a call with
  *   weights, or without, uses (0 where each row is stored as it is computed; work may then be NULL).
@@ -431,8 +432,8 @@ int otpu_attn_shared(const otpu_attn_args* args, otpu_stream_t stream);
  * lower slots), then by weight, the lower slot where weights are equal (a NaN weight counts as the largest).  The j-th slot below budget
  * that goes is overwritten by the j-th slot at or past budget that stays (rows of k and v in place, its
  * weight and position); slots keep no order.  lens_out[b] = min(lens[b], budget); slots from there on get
- * weight 0 and position -1.  T at most 2^30.
- *   k, v [B, T, H] rows of row_bytes bytes (a multiple of 16; strides kb, kt, kh, vb, vt, vh in bytes,
+ * weight 0 and position -1.  T at most 2^30, B * H below 2^22.
+ *   k, v [B, T, H] rows of row_bytes bytes (a multiple of 16, at most 2^20; strides kb, kt, kh, vb, vt, vh in bytes,
  *   multiples of 16); weights fp32 and pos int32 [B, H, T]; weights_out, pos_out and lens_out are the old
  *   arrays or ones that overlap nothing.  work: otpu_kv_evict_work_bytes(...) bytes, 256-byte aligned. */
 typedef struct otpu_evict_args {

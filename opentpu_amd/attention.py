@@ -73,7 +73,8 @@ def shared(q, prefix_k, prefix_v, k, v, lens, *, scale: float | None = None, wei
     query i of sequence b sees the whole prefix and own tokens 0 .. lens[b] - Lq + i.  Returns out
     [B, Lq, Hq, D] in q's type; a query that sees no key gives 0.
 
-    Hq is a multiple of Hkv, D a multiple of 8 up to 256.  scale: D ** -0.5 unless given.  prefix_k and
+    Hq is a multiple of Hkv, D a multiple of 8 up to 256, B * Lq * Hq at most 2^23, P at most 2^30, B * Hkv *
+    ceil(T / 32) below 2^24, tokens less than 2^22 elements apart.  scale: D ** -0.5 unless given.  prefix_k and
     prefix_v may be None, so may k, v and lens together.  weights (float32 [B, Hkv, T], contiguous): each
     own token's softmax weights, summed over the queries and the query heads of its head, are added to
     it.  out: a tensor to write to, which must overlap no input."""
@@ -142,7 +143,7 @@ def evict(k, v, weights, pos, lens, budget: int, recent: int = 0, *, out=None):
     that stay (both in slot order), so slots keep no order of positions.
 
     weights float32 and pos int32 [B, H, T] (contiguous): each slot's accumulated weight (`shared` adds to
-    it) and its token's position.  lens int32 [B].  Returns the new (weights, pos, lens); slots past the new
+    it) and its token's position.  lens int32 [B].  T at most 2^30, B * H below 2^22.  Returns the new (weights, pos, lens); slots past the new
     length have weight 0 and position -1.  out: the three tensors to write them to; (weights, pos, lens)
     themselves may be given."""
     dt, dev, T = k.dtype, k.get_device(), X.torch()

@@ -951,7 +951,8 @@ static int check_sizes(const char* who, int B, int Lq, int Hq, int Hkv, int D, i
     // (a launch holds fewer than 2^32 threads)
     const int64_t rows = (int64_t)B * Lq * Hq;
     if (rows > (1 << 23) || (int64_t)B * Hkv * ((T + 31) / 32) >= (1 << 24))
-        return otpu_fail(OTPU_EINVAL, "%s: %lld rows, %d sequences of %d tokens", who, (long long)rows, B, T);
+        return otpu_fail(OTPU_EINVAL, "%s: %lld rows (at most 2^23), %d x %d caches of %d tokens (below 2^24 pieces of 32)", who,
+                         (long long)rows, B, Hkv, T);
     return OTPU_OK;
 }
 

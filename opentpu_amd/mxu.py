@@ -215,7 +215,7 @@ def norm_quantize(x, gamma, residual=None, *, eps: float = 1e-6, row_mode: bool 
     h = x + residual (fp32), r = 1 / sqrt(mean(h^2) + eps) a row, and the operand of (h * r) * gamma for
     `dot` (an offset a group of 32; row_mode: one): as `fp32.qact` of the fp32 h with rscale r and cscale
     gamma.  x [M, K] float32, bfloat16 or float16, residual of its type (or None), gamma [K]; K a multiple
-    of 32 (a `dot` needs 128).  Returns (operand, h): h in x's type, x itself without a residual.
+    of 32 (a `dot` needs 128) up to 32768, M below 2^22.  Returns (operand, h): h in x's type, x itself without a residual.
     Tensors of the current device.  h: a tensor for the sum, x or residual among them; r: a float32 tensor [M] for the rows' factors."""
     T = X.torch()
     if not NORM_TYPES:
