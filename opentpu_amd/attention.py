@@ -93,24 +93,28 @@ def shared(q, prefix_k, prefix_v, k, v, lens, *, scale: float | None = None, wei
     qs = q.stride()
     if qs[3] != 1:
         _rows("shared", "q", q, dt, (B, Lq, Hq, D), dev)
-    if (k is not None and k.dim() != 4) or (prefix_k is not None and prefix_k.dim() != 3):
-        raise ValueError("shared: a cache has four dimensions, a prefix three")
+    own = pre = (0, 0, 0)
     if k is not None:                                      # (tests in line: the functions say what is wrong)
-        N, Hkv = k.shape[1], k.shape[-2]
-        own, ks, vs = (B, N, Hkv, D), k.stride(), v.stride()
-        if k.dtype != dt or k.shape != own or k.get_device() != dev or ks[3] != 1:
-            _rows("shared", "k", k, dt, own, dev)
+        own = k.shape
+        if len(own) != 4:
+            raise ValueError(f"shared: k is {list(own)}, needs [B, T, Hkv, D]")
+        N, Hkv = own[1], own[2]
+        ks, vs = k.stride(), v.stride()
+        if k.dtype != dt or own[0] != B or own[3] != D or k.get_device() != dev or ks[3] != 1:
+            _rows("shared", "k", k, dt, (B, N, Hkv, D), dev)
         if v.dtype != dt or v.shape != own or v.get_device() != dev or vs[3] != 1:
             _rows("shared", "v", v, dt, own, dev)
         lp = _dense("shared", "lens", lens, T.int32, (B,), dev)
         kp, vp = k.data_ptr(), v.data_ptr()
-    else:
-        Hkv = prefix_k.shape[-2]
     if prefix_k is not None:
-        P, ps, pvs = prefix_k.shape[0], prefix_k.stride(), prefix_v.stride()
-        pre = (P, Hkv, D)
-        if prefix_k.dtype != dt or prefix_k.shape != pre or prefix_k.get_device() != dev or ps[2] != 1:
-            _rows("shared", "prefix_k", prefix_k, dt, pre, dev)
+        pre = prefix_k.shape
+        if len(pre) != 3:
+            raise ValueError(f"shared: prefix_k is {list(pre)}, needs [P, Hkv, D]")
+        if k is None:
+            Hkv = pre[1]
+        P, ps, pvs = pre[0], prefix_k.stride(), prefix_v.stride()
+        if prefix_k.dtype != dt or pre[1] != Hkv or pre[2] != D or prefix_k.get_device() != dev or ps[2] != 1:
+            _rows("shared", "prefix_k", prefix_k, dt, (P, Hkv, D), dev)
         if prefix_v.dtype != dt or prefix_v.shape != pre or prefix_v.get_device() != dev or pvs[2] != 1:
             _rows("shared", "prefix_v", prefix_v, dt, pre, dev)
         pk, pv = prefix_k.data_ptr(), prefix_v.data_ptr()
@@ -125,7 +129,7 @@ def shared(q, prefix_k, prefix_v, k, v, lens, *, scale: float | None = None, wei
         return out
     if N == 1 or P == 1 or (qs[0] | qs[1] | qs[2] | ps[0] | ps[1] | pvs[0] | pvs[1] | ks[0] | ks[1] | ks[2] | vs[0] | vs[1] | vs[2]
                             | os[0] | os[1] | os[2]) & 7:
-        qs, os, own, pre = _used(q.shape, qs), _used(q.shape, os), (B, N, Hkv), (P, Hkv)
+        qs, os = _used(q.shape, qs), _used(q.shape, os)
         ks, vs, ps, pvs = _used(own, ks), _used(own, vs), _used(pre, ps), _used(pre, pvs)
     nbytes = _attn_bytes(B, Lq, Hq, Hkv, D, P, N, weights is not None)
     work = q.new_empty((nbytes // 2 + 1,))                 # (of q's type: the least work for the host)
@@ -147,12 +151,15 @@ def evict(k, v, weights, pos, lens, budget: int, recent: int = 0, *, out=None):
     length have weight 0 and position -1.  out: the three tensors to write them to; (weights, pos, lens)
     themselves may be given."""
     dt, dev, T = k.dtype, k.get_device(), X.torch()
-    budget, recent = _count(budget), _count(recent)
+    if type(budget) is not int or type(recent) is not int or (budget | recent) >> 31:
+        budget, recent = _count(budget), _count(recent)
     if k.dim() != 4 or dev < 0 or dt not in _types():
         raise ValueError(f"evict: k is {dt} {list(k.shape)} on {k.device}, needs [B, T, H, D] in bfloat16, float16 or float32")
     B, N, H, D = k.shape
     e = k.element_size()
-    ks, vs = (_used(k.shape, _rows("evict", name, t, dt, (B, N, H, D), dev, True)) for name, t in (("k", k), ("v", v)))
+    ks, vs = _rows("evict", "k", k, dt, (B, N, H, D), dev, True), _rows("evict", "v", v, dt, (B, N, H, D), dev, True)
+    if e * (ks[0] | ks[1] | ks[2] | vs[0] | vs[1] | vs[2]) & 15:
+        ks, vs = _used(k.shape, ks), _used(k.shape, vs)
     slots = (B, H, N)
     if out is None:
         out = (T.empty_like(weights), T.empty_like(pos), T.empty_like(lens))

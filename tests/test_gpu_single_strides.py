@@ -65,3 +65,15 @@ def test_evict(T, size):
     want = attention.evict(k1, v1, w, pos, lens, n // 2, 1)
     got = attention.evict(k2, v2, w, pos, lens, n // 2, 1)
     assert T.equal(k1, k2) and T.equal(v1, v2) and all(T.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_prefix_or_a_cache_alone(T):
+    """One token of the one without the other, and rows of an odd pitch."""
+    from opentpu_amd import attention
+    rng = np.random.default_rng(4)
+    q, p, k = (T.from_numpy(rng.standard_normal(s).astype(np.float32)).half().cuda() for s in ((2, 1, 2, 64), (1, 2, 64), (2, 1, 2, 64)))
+    lens = T.ones((2,), dtype=T.int32, device="cuda")
+    for x in (q, odd(T, q)):
+        assert T.equal(attention.shared(x, p, p, None, None, None), p.expand(2, 1, 2, 64))
+        assert T.equal(attention.shared(x, None, None, k, k, lens), k)
+        assert T.equal(attention.shared(x, odd(T, p), p, None, None, None), p.expand(2, 1, 2, 64))
