@@ -400,8 +400,9 @@ int otpu_norm_qact(const void* x, int64_t ldx, const void* res, int64_t ldr, int
  *   tokens 0 .. lens[b] - Lq + i.  Head h of q reads head h / (Hq / Hkv) of the keys.
  *   out [B, Lq, Hq, D] = sum softmax(scale q k) v; 0 where a query sees no key.  weights (may be NULL)
  *   [B, Hkv, T] fp32: the own tokens' softmax weights, summed over the Lq queries and the head's Hq / Hkv
- *   query heads, are added to it.  dtype OTPU_BF16 or OTPU_F16 for q, caches and out; sums, maxima and
- *   weights fp32.  D a multiple of 8, at most 256; scale from 5e-46 to 1e30; addresses 16-byte aligned, strides
+ *   query heads, are added to it.  dtype OTPU_BF16 or OTPU_F16 for q, caches and out; scores, sums,
+ *   maxima and what is added to `weights` fp32; for its product with the values each softmax weight is rounded
+ *   to dtype (its sum is not), about as large an error as the output's own rounding.  D a multiple of 8, at most 256; scale from 5e-46 to 1e30; addresses 16-byte aligned, strides
  *   multiples of 8, tokens less than 2^22 elements apart.  P or T may be 0 (its operands NULL).
  *   Limits: B * Lq * Hq at most 2^23 rows, P at most 2^30, B * Hkv * ceil(T / 32) below 2^24 (one cache of
  *   2^29 - 32 tokens; 256 sequences on 8 heads of 262112).

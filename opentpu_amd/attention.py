@@ -71,7 +71,8 @@ def shared(q, prefix_k, prefix_v, k, v, lens, *, scale: float | None = None, wei
     """Attention of q [B, Lq, Hq, D] over the shared prefix [P, Hkv, D] and each sequence's own cache
     k, v [B, T, Hkv, D], of which lens [B] (int32) tokens are in use, the Lq newest the queries' own:
     query i of sequence b sees the whole prefix and own tokens 0 .. lens[b] - Lq + i.  Returns out
-    [B, Lq, Hq, D] in q's type; a query that sees no key gives 0.
+    [B, Lq, Hq, D] in q's type; a query that sees no key gives 0.  Scores, maxima and sums are float32; for its product
+    with the values each softmax weight is rounded to q's type, about as large an error as the output's own rounding.
 
     Hq is a multiple of Hkv, D a multiple of 8 up to 256, B * Lq * Hq at most 2^23, P at most 2^30, B * Hkv *
     ceil(T / 32) below 2^24, tokens less than 2^22 elements apart.  scale: D ** -0.5 unless given.  prefix_k and
@@ -142,13 +143,13 @@ def shared(q, prefix_k, prefix_v, k, v, lens, *, scale: float | None = None, wei
 
 def evict(k, v, weights, pos, lens, budget: int, recent: int = 0, *, out=None):
     """Frees slots of the caches k, v [B, T, H, D] in place: where lens[b] > budget, each head keeps `budget`
-    slots, those of its `recent` newest positions first (of more than `budget` the lower slots), then those of the largest accumulated weights, the
-    lower slot where they are equal.  Slots below budget that go are overwritten by the slots past it
+    slots, those of its `recent` newest positions first (of more than `budget` the lower slots), then those of the
+    largest accumulated weights, the lower slot where they are equal.  Slots below budget that go are overwritten by the slots past it
     that stay (both in slot order), so slots keep no order of positions.
 
     weights float32 and pos int32 [B, H, T] (contiguous): each slot's accumulated weight (`shared` adds to
-    it) and its token's position.  lens int32 [B].  T at most 2^30, B * H below 2^22.  Returns the new (weights, pos, lens); slots past the new
-    length have weight 0 and position -1.  out: the three tensors to write them to; (weights, pos, lens)
+    it) and its token's position.  lens int32 [B].  T at most 2^30, B * H below 2^22.  Returns the
+    new (weights, pos, lens); slots past the new length have weight 0 and position -1.  out: the three tensors to write them to; (weights, pos, lens)
     themselves may be given."""
     dt, dev, T = k.dtype, k.get_device(), X.torch()
     if type(budget) is not int or type(recent) is not int or (budget | recent) >> 31:

@@ -9,10 +9,11 @@
 //                    weights from their scores
 //   weights_kernel   the weights where many rows would make the scores large: from the keys again
 //
-// What bounds it, by sizes (bf16, 16 heads on 8, heads of 128): own keys and a prefix under few rows by
-// memory (64 sequences on 1024 own tokens each 5.8 TB/s, 16 rows on 65536 shared tokens 5.3); many rows by
-// the matrix units at the clock that their power leaves (8 x 512 queries on 8192 tokens 930-990 TFLOP/s; a
-// library product of 8192^3 reaches 1177); the smallest calls by launches (two, 7 us).
+// What bounds it, by sizes (bf16, 16 heads on 8, heads of 128; whole calls, one after another): own keys and a
+// prefix under few rows by memory (64 sequences on 1024 own tokens each 52 us, 5.2 TB/s; 16 on 65536 shared
+// tokens 61 us, 4.4); many rows by the matrix units at the clock that their power leaves (8 x 512 queries on 8192
+// tokens 297 us, 985 TFLOP/s; a library product of 8192^3 reaches 1190); the smallest calls by launches (one
+// sequence on 128 shared tokens and up to 64 own: two, 8.5 us).
 #include "otpu_common.h"
 
 namespace otpu {
@@ -308,7 +309,8 @@ template <class E, int DP, bool FULL>
 __device__ __forceinline__ void store_part(const AttnArgs& a, const Acc<DP>& c, float l, const Part& p) {
     if (!p.valid) return;
     const int hh = (threadIdx.x >> 5) & 1;
-    // (a join of 4096 x 16 rows takes 17 us, a launch 2.5; heads of 256 have no registers for it)
+    // (4096 queries of 16 heads on their own keys through a join: 118 us, without it 104; heads of 256 have no
+    // registers for it)
     if (DP <= 128 && a.whole) {
         char* const out = out_row(a, p.at);
         const float il = l == 0.f ? 0.f : 1.f / l;
@@ -387,7 +389,7 @@ __device__ __forceinline__ void clear_lds(char* lds, int bytes) {
 }
 
 // Two workgroups a CU, a wave of each on a SIMD: the one's products fill the other's arithmetic in part (MFMA
-// busy 54% of the cycles at 1.9 GHz).  Two groups of waves that alternate at barriers instead, products beside
+// busy 51 to 56% of the cycles, at 1.9 GHz).  Two groups of waves that alternate at barriers instead, products beside
 // softmax: 780 TFLOP/s against 990.  Keys loaded two steps ahead: no change, the loads are not waited for; four
 // places of 32 keys in place of two of 64: the same to 10% slower, for the barriers.
 // BOTH: the prefix's keys, then the own ones (p's), as one row of steps.
@@ -539,11 +541,11 @@ __device__ __forceinline__ void keys_part(const AttnArgs& a, char* lds, const Pa
 // the XCDs and a split's row tiles next to each other, so that one L2 serves them the same keys.  (Both
 // kinds in turn, for the products of the one beside the loads of the other, takes that sharing from the
 // row tiles: 256 sequences on 131072 tokens 743 us, one kind after the other 526.)  Own: (head, row tile,
-// sequence, split), without a prefix a sequence's last rows first: they see the most keys (64 x 512 queries on
-// their own 174 -> 171 us; behind a prefix no gain, and heads of 256 lose 2%).  Where a prompt's row tiles all have
+// sequence, split), without a prefix a sequence's last rows first: they see the most keys (16384 queries on
+// their own 1153 -> 1038 us, 4096 104 -> 96, 64 x 512 no difference; behind a prefix no gain, and heads of 256 lose 2%).  Where a prompt's row tiles all have
 // their places at once and some CUs two, the first on the CUs (`half` a head) go from those of most keys
-// down and the second from the least up, so that each CU has the same work: 4096 queries on their own keys
-// 118 -> 104 us, 4 x 1024 42 -> 33.
+// down and the second from the least up, so that each CU has the same work: 8 x 512 queries on their own keys
+// 27 -> 23 us, 4 x 1024 40 -> 32, 4096 96 -> 94.
 // The part of workgroup x of its kind; `wrow`: this lane's row in a tile of bm rows; false: no key
 __device__ __forceinline__ bool find_part(const AttnArgs& a, bool own, uint32_t x, int bm, int wrow, Part& p) {
     const int R = a.Lq * a.G;
@@ -622,7 +624,7 @@ __global__ __launch_bounds__(NW * 64, DP <= 128 ? 2 : 1) void segment_kernel(Att
 
 // A sequence's tile of 128 rows against the prefix and its own keys (a kernel of its own: in segment_kernel its
 // addresses would not stay in scalar registers).  16 x 256 queries on 1024 shared tokens and their own, 16 heads
-// on 8 of 128: 76 -> 51 us; 4 x 2048 on 2048 274 -> 230, 8 x 512 on 8192 302 -> 291.
+// on 8 of 128: 77 -> 51 us; 4 x 2048 on 2048 276 -> 229, 8 x 512 on 8192 and up to 1024 own tokens 318 -> 297.
 template <class E, int DP, bool FULL>
 __global__ __launch_bounds__(NW * 64, 2) void both_kernel(AttnArgs a) {
     __shared__ __attribute__((aligned(16))) char lds[Shape<DP>::ROWS_LDS];
@@ -776,11 +778,13 @@ __global__ __launch_bounds__(256) void combine_kernel(AttnArgs a, int nw) {
     if (a.lse && d == 0) a.lse[row] = m + __builtin_log2f(l);
 }
 
-// Own key weights where R > 32 rows' scores would take more than half of the keys' bytes: a workgroup takes 32
-// keys of a (sequence, head), its waves the rows in tiles of 32 by turns.  As in `scores` a lane has one row
+// Own key weights where R > 32 rows see a (sequence, head)'s keys (up to 32 their scores are kept: at 32 half of the
+// keys' bytes for heads of 128, all of them for 64, 8 times them for 8): a workgroup takes 32 keys of a (sequence, head), its waves the rows in tiles of 32 by turns.  As in `scores` a lane has one row
 // and 16 of the keys, so that the row's lse is its own and the sums over row tiles stay in registers; lanes and
-// waves are summed once at the end, in one order, and nothing is atomic.  (82 x 13 queries for 5 heads on 786
-// own tokens 32 us; 128 keys a workgroup, so that the queries are read less often, 39: fewer waves a SIMD.)
+// waves are summed once at the end, in one order, and nothing is atomic.  (82 x 13 queries, 15 heads on 3 of 128, on
+// up to 786 own tokens 24 us.  128 keys a workgroup, each wave all rows for its own 32, read the queries a quarter as
+// often with fewer waves a SIMD: the call 56 us against 58, 16 x 64 queries on 2048 tokens 103 against 118, but 8 x 512
+// on up to 1024 102 against 90.)
 template <class E, int DP, bool FULL>
 __global__ __launch_bounds__(NW * 64) void weights_kernel(AttnArgs a) {
     constexpr int KS = DP / 16;
@@ -855,13 +859,15 @@ static Plan plan(int B, int Lq, int Hq, int Hkv, int D, int P, int T, bool weigh
     const int R = Lq * (Hq / Hkv);
     const int64_t M = (int64_t)B * R, slots = 2 * (int64_t)otpu_cu_count();
     p.rows = (int64_t)B * Lq * Hq;
-    // (own keys of up to 64 rows: two tiles of 32 read them from the L2; 16 x 24 queries for 2 heads on 200 own
-    // tokens 18.4 us, a tile of 128 21.4.  A prefix: no difference.)
+    // (own keys of up to 64 rows: two tiles of 32 read them from the L2; 16 x 24 queries, 4 heads on 2, on 200 own
+    // tokens 9.2 us, a tile of 128 12.8.  A prefix: no difference.)
     p.rows_p = M <= 32 ? 32 : 32 * NW;
     p.rows_o = R <= 64 ? 32 : 32 * NW;
     const int64_t gp = (int64_t)Hkv * ((M + p.rows_p - 1) / p.rows_p);
     const int64_t go = (int64_t)B * Hkv * ((R + p.rows_o - 1) / p.rows_o);
-    // Splits: as many as fill the places of the CUs, of `least` keys or more.
+    // Splits: as many as fill the places of the CUs, of `least` keys or more.  (Two places a CU, also for the copy of
+    // 256 columns, which has one: 64 sequences on 16384 tokens and up to 1024 own, heads of 256, 121 us, counted as one
+    // 136; 16 on 65536 125 against 110.)
     auto splits = [&](int64_t groups, int64_t keys, int64_t least) {
         if (keys <= 0 || groups <= 0) return (int64_t)0;
         const int64_t s = (slots + groups - 1) / groups, most = (keys + least - 1) / least;
@@ -873,9 +879,9 @@ static Plan plan(int B, int Lq, int Hq, int Hkv, int D, int P, int T, bool weigh
     if (p.rows_p > 32 && s > 1) {
         // A tile of 128 rows writes 64 KB of partials a split, read once more, where another split saves
         // each workgroup steps: the sum is least near sqrt(P / (2 groups)) (64 sequences on 4096 tokens, 8
-        // groups: 8, 16 and 32 splits 18.6, 15.1 and 17.3 us; on 16384 16, 32 and 64 33.6, 28.3 and 31.2).
+        // groups: 8, 16 and 32 splits 19.0, 15.7 and 16.7 us; on 16384 16, 32 and 64 29.8, 25.4 and 29.8).
         // Half of that beside own keys that fill the CUs: there the steps' latency does not count (64
-        // sequences on 16384, up to 1024 own tokens: 32 splits 64 us, 16 59, 8 80).
+        // sequences on 16384, up to 1024 own tokens: 32 splits 65 us, 16 62, 8 71).
         const int64_t r = (int64_t)__builtin_ceil(__builtin_sqrt((double)P / (2.0 * (double)gp)));
         if (r < s) s = p.no >= slots / 2 ? (r + 1) / 2 : r;
     }

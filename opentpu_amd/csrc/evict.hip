@@ -9,8 +9,8 @@
 //                         rows of k and v
 //   evict_move_kernel     more rows of k and v, and the slots that are free
 //
-// The moves are bound by memory (64 x 8 caches of 2048 slots cut to 1000: 268 MB read and written, 64 us with
-// the selection, 4.2 TB/s; a copy reaches 5.1).  The selection is a chain of a few trips to memory, three
+// The moves are bound by memory (64 x 8 caches of 2048 slots cut to 1000: 268 MB read and written, 65 us after a
+// selection of 15, 4.1 TB/s; a copy reaches 5.1).  The selection is a chain of a few trips to memory, three
 // passes over keys in registers with three barriers each, and a scan: 8 us for 256 caches of 1024 slots with
 // the launch, 27 for caches of 32768, where one workgroup's instructions bound it.
 #include "otpu_common.h"
@@ -21,7 +21,10 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
 constexpr int EW = 1024;                     // threads of a selecting workgroup
 constexpr int BINS = 2048;
-constexpr int HERE = 64;                     // moves that the selecting workgroup makes itself
+// Moves that the selecting workgroup makes itself, with the free slots' clearing: a launch less, whatever the slots.
+// 256 caches of 16-bit rows of 64 cut to 64 slots, of 1024: 9.4 us, moved and cleared by the second kernel 11.9; of
+// 32768 slots 36.4 and 41.0; 8 caches of 32768 22.9 and 24.3.
+constexpr int HERE = 64;
 
 struct EvictArgs {
     char* k; int64_t kb, kt, kh;             // byte strides of sequence, slot, head
@@ -274,8 +277,8 @@ __global__ __launch_bounds__(256) void evict_lens_kernel(EvictArgs a) { store_le
 __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
     const int bh = blockIdx.x, b = bh / a.H, h = bh - b * a.H;
     if (bh == 0 && blockIdx.y == 0 && a.ln == a.lens) store_lens(a);
-    // the slots past the new length (the same from the old length and the new one).  Here and not in the
-    // selection: one workgroup's stores to most of a long cache would make everything wait
+    // the slots past the new length (the same from the old length and the new one).  Here, where there is a second
+    // launch: the selection need not wait for its one workgroup's stores (32 caches of 32768 slots cut to 4096 46 -> 44 us)
     const int left = min(min(max(a.lens[b], 0), a.T), a.budget);
     for (int64_t t = left + (int)(blockIdx.y * 256 + threadIdx.x); t < a.T; t += 256 * (int64_t)gridDim.y) {
         a.wn[(int64_t)bh * a.T + t] = 0.f;
